@@ -22,6 +22,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "gbx.h")
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 30
 EMBED_BAD_ID, EMBED_BAD_POS, EMBED_TIMEOUT = 1, 2, 4
+KV_BAD_PAGE, KV_BAD_LEN, KV_BAD_PAIR, VERIFY_BAD_ID, VERIFY_BAD_ROW = 8, 16, 32, 64, 128
 
 STATUS = {0: "GBX_OK", 1: "GBX_EINVAL", 2: "GBX_EDTYPE", 3: "GBX_ERANGE", 4: "GBX_ECUDA",
           5: "GBX_EIO", 6: "GBX_ENOTFOUND", 7: "GBX_ENOMEM"}
@@ -68,9 +69,16 @@ SIGNATURES = {
     "gbx_linear": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _vp, _vp],
     "gbx_linear_splitk": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _i64, _vp, _vp],
     "gbx_linear_splitk_noalloc": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _int, _vp, _vp],
+    "gbx_kv_append": [_vp, _int, _vp, _int, _vp, _vp, _int, _int, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
+    "gbx_kv_read": [_vp, _int, _vp, _int, _vp, _vp, _int, _int, _vp, _vp, _i64, _vp, _vp],
+    "gbx_kv_copy_pages": [_vp, _vp, _vp, _int, _vp, _vp],
+    "gbx_attn_cached": [_vp, _int, _vp, _vp, _i64, _vp, _int, _vp, _vp, _int, _int, _int, _f, _vp, _vp, _i64, _vp, _i64,
+                        _vp, _vp],
+    "gbx_attn_cached_workspace": [_vp, _int, _int, _int, _int],
+    "gbx_verify_tokens": [_vp, _vp, _vp, _vp, _i64, _int, _int, ctypes.c_double, _vp, _vp, _vp, _vp, _vp],
 }
 _RESTYPES = {"gbx_status_string": ctypes.c_char_p, "gbx_last_error": ctypes.c_char_p,
-             "gbx_set_first_wait_limit": ctypes.c_uint64}
+             "gbx_set_first_wait_limit": ctypes.c_uint64, "gbx_attn_cached_workspace": _i64}
 
 _lib = None
 
@@ -278,3 +286,129 @@ def attn_fused(q_hi, q_lo, k_hi, k_lo, v_hi, v_lo, out, *, ld, ld_out, B, S, H, 
     """Self-attention of every head in one fused launch (tf32 pairs in; see gbx.h)."""
     _check(lib().gbx_attn_fused(_p(q_hi), _p(q_lo), _p(k_hi), _p(k_lo), ld, _p(v_hi), _p(v_lo), _p(out), _p(out_lo),
                                 ld_out, B, S, H, hd, scale, 1 if causal else 0, _p(err_flag), _stream(stream)))
+
+
+class _KVCacheStruct(ctypes.Structure):
+    """gbx_kv_cache of gbx.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("layers", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("heads", ctypes.c_int32), ("hd", ctypes.c_int32)]
+
+
+class KVCache:
+    """Paged 8-bit key/value cache (gbx_kv_cache): ``KVCache(layers=, pages=,
+    heads=, page=, hd=)`` allocates its four tensors on `device`;
+    ``KVCache(k=, v=, k_scale=, v_scale=)`` wraps tensors of the layout gbx.h
+    gives.  The tensors stay reachable as ``.k .v .k_scale .v_scale``."""
+
+    def __init__(self, *, layers=None, pages=None, heads=None, page=None, hd=None, k=None, v=None, k_scale=None,
+                 v_scale=None, device="cuda"):
+        import torch
+        if k is None:
+            if page not in (16, 32, 64, 128):
+                raise ValueError(f"KVCache: {page} tokens per page (16, 32, 64 or 128)")
+            k = torch.empty((layers, pages, heads, page, hd), dtype=torch.int8, device=device)
+            v = torch.empty((layers, pages, heads, page // 16, hd, 16), dtype=torch.int8, device=device)
+            k_scale = torch.empty((layers, pages, heads), dtype=torch.float32, device=device)
+            v_scale = torch.empty((layers, pages, heads), dtype=torch.float32, device=device)
+        layers, pages, heads, page, hd = k.shape
+        want = {"k": (k, torch.int8, (layers, pages, heads, page, hd)),
+                "v": (v, torch.int8, (layers, pages, heads, page // 16, hd, 16)),
+                "k_scale": (k_scale, torch.float32, (layers, pages, heads)),
+                "v_scale": (v_scale, torch.float32, (layers, pages, heads))}
+        for name, (t, dtype, shape) in want.items():
+            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != k.device:
+                raise ValueError(f"KVCache: {name} must be a contiguous {dtype} tensor {shape} on {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.layers, self.pages, self.heads, self.page, self.hd = layers, pages, heads, page, hd
+        self.device = k.device
+        self._c = _KVCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, layers, page,
+                                 heads, hd)
+        self._ref = ctypes.byref(self._c)
+
+
+def _int32(**tensors):
+    """The index arrays of the cache calls, where they are tensors: int32, contiguous."""
+    for name, t in tensors.items():
+        if t is not None and not isinstance(t, int) and (str(t.dtype) != "torch.int32" or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 tensor")
+
+
+class _on_device:
+    """The launch's device made current: a kernel runs where its tensors are,
+    whichever device the caller has selected."""
+
+    def __init__(self, device):
+        self.guard = None
+        if device is not None and device.type == "cuda":
+            import torch
+            if device.index is not None and device.index != torch.cuda.current_device():
+                self.guard = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_new=None, k_lo=None, v_lo=None,
+              err_flag=None, stream=None):
+    """Appends row (b, i), i < n_new[b], of k and v (row stride ld) as token
+    kv_len[b] - n_new[b] + i of sequence b.  max_pages: the table's row length
+    (its last dimension when it is a tensor)."""
+    _int32(table=table, kv_len=kv_len, n_new=n_new)
+    with _on_device(cache.device):
+        _check(lib().gbx_kv_append(cache._ref, layer, _p(table), _max_pages(table, max_pages), _p(kv_len), _p(n_new), B, S,
+                                   _p(k), _p(k_lo), _p(v), _p(v_lo), ld, _p(err_flag), _stream(stream)))
+
+
+def _max_pages(table, max_pages):
+    return table.shape[-1] if max_pages is None else max_pages
+
+
+def kv_read(cache, layer, table, kv_len, k_out, v_out, *, B, S, ld, max_pages=None, n=None, err_flag=None, stream=None):
+    """The fp32 values of each sequence's last n[b] tokens (the mirror of kv_append)."""
+    _int32(table=table, kv_len=kv_len, n=n)
+    with _on_device(cache.device):
+        _check(lib().gbx_kv_read(cache._ref, layer, _p(table), _max_pages(table, max_pages), _p(kv_len), _p(n), B, S,
+                                 _p(k_out), _p(v_out), ld, _p(err_flag), _stream(stream)))
+
+
+def kv_copy_pages(cache, src, dst, *, n, err_flag=None, stream=None):
+    """Page dst[i] becomes page src[i], i < n, in every layer."""
+    _int32(src=src, dst=dst)
+    with _on_device(cache.device):
+        _check(lib().gbx_kv_copy_pages(cache._ref, _p(src), _p(dst), n, _p(err_flag), _stream(stream)))
+
+
+def attn_cached_workspace(cache, *, B, S, H, max_pages) -> int:
+    """Floats of workspace attn_cached can use for these sizes (0: none)."""
+    with _on_device(cache.device):
+        n = lib().gbx_attn_cached_workspace(cache._ref, B, S, H, max_pages)
+    if n < 0:
+        _check(-n)
+    return n
+
+
+def attn_cached(cache, layer, q, out, table, kv_len, *, B, S, H, ld, ld_out, scale, max_pages=None, n_new=None, q_lo=None,
+                out_lo=None, workspace=None, workspace_floats=None, err_flag=None, stream=None):
+    """Attention of S rows per sequence over the cached tokens (see gbx.h)."""
+    _int32(table=table, kv_len=kv_len, n_new=n_new)
+    if workspace_floats is None:
+        workspace_floats = workspace.numel() if hasattr(workspace, "numel") else 0
+    with _on_device(cache.device):
+        _check(lib().gbx_attn_cached(cache._ref, layer, _p(q), _p(q_lo), ld, _p(table), _max_pages(table, max_pages),
+                                     _p(kv_len), _p(n_new), B, S, H, scale, _p(out), _p(out_lo), ld_out, _p(workspace),
+                                     workspace_floats, _p(err_flag), _stream(stream)))
+
+
+def verify_tokens(logits, draft_ids, out_ids, n_accepted, *, B, n_draft, vocab, temperature=0.0, uniforms=None,
+                  draft_logits=None, draft_len=None, err_flag=None, stream=None):
+    """Accepts drafted tokens against the target's logits and picks the next token (see gbx.h)."""
+    _int32(draft_ids=draft_ids, out_ids=out_ids, n_accepted=n_accepted, draft_len=draft_len)
+    with _on_device(getattr(logits, "device", None)):
+        _check(lib().gbx_verify_tokens(_p(logits), _p(draft_logits), _p(draft_ids), _p(draft_len), B, n_draft, vocab,
+                                       float(temperature), _p(uniforms), _p(out_ids), _p(n_accepted), _p(err_flag),
+                                       _stream(stream)))

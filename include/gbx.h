@@ -441,6 +441,160 @@ int gbx_attn_fused(const float* q_hi, const float* q_lo, const float* k_hi, cons
                    const float* v_hi, const float* v_lo, float* out, float* out_lo, int64_t ld_out, int B, int S,
                    int H, int hd, float scale, int causal, int* err_flag, gbx_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Cached generation: a paged key/value cache in 8 bits, the attention that
+ * reads it, copies of its pages, and the verification of drafted tokens.  No
+ * counterpart in the reference, whose generate loop runs the whole prefix
+ * again for every token (transformer.cu:986-1036).
+ * ------------------------------------------------------------------------ */
+
+/*
+ * The cache of `layers` layers, as the caller allocated it (device memory;
+ * the struct itself is host memory, read during the call only):
+ *   k        int8  [layers][pages][heads][page][hd]
+ *   v        int8  [layers][pages][heads][page / 16][hd][16]   (16 tokens innermost)
+ *   k_scale  float [layers][pages][heads]      (v_scale likewise)
+ * A value is code * scale: one scale for each page of tokens and head, codes
+ * in [-127, 127].  `page` (tokens per page) is 16, 32, 64 or 128; hd is a
+ * multiple of 16 up to 128; k and v are 16-byte aligned.  No initialisation
+ * is needed: nothing reads a slot before it is appended to.
+ *
+ * Every call addresses tokens through `table` (int32 [B][max_pages], device):
+ * token t of sequence b is in page table[b*max_pages + t / page], slot
+ * t % page.  kv_len[b] (device) counts sequence b's tokens INCLUDING the
+ * call's own, and row (b, i) of a call's S rows per sequence is token
+ * kv_len[b] - n_new[b] + i, for i < n_new[b]; n_new NULL means S for every
+ * sequence.  Rows i >= n_new[b] are neither read nor written.
+ */
+typedef struct gbx_kv_cache {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t pages;
+    int32_t layers;
+    int32_t page;
+    int32_t heads;
+    int32_t hd;
+} gbx_kv_cache;
+
+/* Bits OR-ed into *err_flag (device int32; may be NULL) by the calls below.
+ * GBX_KV_BAD_PAGE: a page outside [0, pages); its tokens are skipped (not
+ *   written, not attended to).
+ * GBX_KV_BAD_LEN: n_new outside [0, S], or kv_len outside
+ *   [n_new, max_pages * page]; the sequence is skipped.
+ * GBX_KV_BAD_PAIR: a page copy whose target is another pair's source or an
+ *   earlier pair's target; the copy is skipped.
+ * GBX_VERIFY_BAD_ID: a drafted id outside [0, vocab); it is rejected.
+ * GBX_VERIFY_BAD_ROW: a logits row without a usable maximum (a NaN, a +inf,
+ *   or nothing above -inf), or draft_len outside [0, n_draft]. */
+enum { GBX_KV_BAD_PAGE = 8, GBX_KV_BAD_LEN = 16, GBX_KV_BAD_PAIR = 32, GBX_VERIFY_BAD_ID = 64, GBX_VERIFY_BAD_ROW = 128 };
+
+/*
+ * Appends the call's tokens to layer `layer`.  Row (b, i)'s keys of head h
+ * are k_hi[(b*S + i)*ld + h*hd + .] + k_lo[same] (a tf32 pair, as gbx_linear
+ * writes it; the *_lo planes may be NULL), its values likewise: the K and V
+ * column blocks of the QKV output, read as they lie.  For each page touched
+ * and each head, with a = the largest |x| of the call's tokens in that page:
+ *   s_new = a / 127 (to nearest; 0 when a < 2^-100)
+ *   s     = the page's first new slot is 0 ? s_new : max(stored scale, s_new)
+ *   x  ->  the integer nearest to x / s (ties to even); s == 0: 0
+ * and where s grew, codes c of the page's earlier slots become the integer
+ * nearest to c * stored / s.  A value is therefore within s/2 of its input,
+ * plus s/2 for each later growth of its page's scale.  A NaN or an infinity
+ * among the new values makes the page's scale NaN for that head, so that
+ * every later read of that page and head gives NaN until it is started anew.
+ * Exact arithmetic, so the result does not depend on the launch.  Pages that
+ * two sequences of one call both append to are the caller's mistake (their
+ * bytes are then unspecified).
+ */
+int gbx_kv_append(const gbx_kv_cache* cache_host, int layer, const int32_t* table, int max_pages,
+                  const int32_t* kv_len, const int32_t* n_new, int B, int S, const float* k_hi, const float* k_lo,
+                  const float* v_hi, const float* v_lo, int64_t ld, int* err_flag, gbx_stream_t stream);
+
+/*
+ * The values the cache stands for, in fp32 (as gbx_dequant is for tensors):
+ * row (b, i)'s k_out[(b*S + i)*ld + h*hd + .] = code * scale of token
+ * kv_len[b] - n[b] + i, for i < n[b] (n NULL: S); other rows are left as they
+ * were.  k_out or v_out may be NULL.  The mirror of gbx_kv_append.
+ */
+int gbx_kv_read(const gbx_kv_cache* cache_host, int layer, const int32_t* table, int max_pages,
+                const int32_t* kv_len, const int32_t* n, int B, int S, float* k_out, float* v_out, int64_t ld,
+                int* err_flag, gbx_stream_t stream);
+
+/*
+ * Copies n pages in every layer, keys, values and scales: page dst[i] becomes
+ * page src[i] (device arrays).  For forks (the shared, partly filled last
+ * page) and for compaction.  A pair with src[i] == dst[i] does nothing.  The
+ * copies run in no order, so no target may be another pair's source or
+ * target: a pair whose target is a source of another pair, or the target of
+ * an earlier one, is skipped and reported (GBX_KV_BAD_PAIR).
+ */
+int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* src, const int32_t* dst, int n, int* err_flag,
+                      gbx_stream_t stream);
+
+/*
+ * Attention of the call's S rows per sequence over layer `layer` of the
+ * cache (which holds the rows' own tokens already: gbx_kv_append first):
+ *   out[(b*S + i)*ld_out + h*hd + .] = sum_t w_t v_t,
+ *   w = softmax over t <= kv_len[b] - n_new[b] + i of q . k_t / scale
+ * H query heads; head h reads key head h / (H / heads) (H a multiple of
+ * heads).  q: row (b, i) at q_hi + q_lo [(b*S + i)*ld + h*hd + .] (q_lo may
+ * be NULL).  out_lo NULL: out receives the fp32 result; otherwise out and
+ * out_lo its tf32 pair, the x operand of the output projection.  S = 1 is a
+ * decode step, a few rows score drafted tokens, many are the next chunk of a
+ * prompt.  The codes enter the tensor cores exactly, the queries and weights
+ * as pairs of 11-bit halves, the sums are fp32: the result is that of fp32
+ * attention over the cached values to within rounding (about 2^-21 of the
+ * scores' and values' magnitudes).  A page read by a valid row whose scale
+ * is NaN gives NaN; a row that sees no page that can be read gives 0.  out
+ * and out_lo must overlap neither each other nor q.
+ *
+ * workspace: device floats, at least gbx_attn_cached_workspace(...) of them
+ * (0: none needed, NULL will do); long caches read by few heads are cut into
+ * pieces whose partial results meet there.  NULL or too few floats: the call
+ * runs without the cut.  Calls that can overlap on the GPU need workspaces of
+ * their own.  Nothing in it is kept between calls.
+ */
+int gbx_attn_cached(const gbx_kv_cache* cache_host, int layer, const float* q_hi, const float* q_lo, int64_t ld,
+                    const int32_t* table, int max_pages, const int32_t* kv_len, const int32_t* n_new, int B, int S,
+                    int H, float scale, float* out, float* out_lo, int64_t ld_out, float* workspace,
+                    int64_t workspace_floats, int* err_flag, gbx_stream_t stream);
+
+/* Floats of workspace gbx_attn_cached uses for these sizes on the current
+ * device (0: none), or a negative GBX_E* code. */
+int64_t gbx_attn_cached_workspace(const gbx_kv_cache* cache_host, int B, int S, int H, int max_pages);
+
+/*
+ * Verification of drafted tokens (speculative decoding) beside
+ * gbx_select_tokens: B sequences, up to n_draft drafts each (draft_len[b] of
+ * them; NULL: n_draft).  logits [B][n_draft + 1][vocab] are the target's, row
+ * i the distribution of the token at draft position i (row draft_len[b]
+ * follows the last draft).  With p_i = softmax(logits_i / T), q_i =
+ * softmax(draft_logits_i / T) ([B][n_draft][vocab]; NULL: the drafts were
+ * picked without chance, q_i is 1 at draft_ids[b][i]) and u = uniforms[b]
+ * ([B][n_draft + 1] doubles in [0, 1)):
+ *   draft i is accepted while u[i] * q_i(d_i) < p_i(d_i)
+ *   after the first rejection, at i: the next token is the first j with
+ *     cum_j > u[n_draft] * cum_vocab, cum the running sum of max(p_i - q_i, 0)
+ *     (of p_i itself should that sum be 0)
+ *   all accepted: the same with p_draft_len[b]
+ * so the tokens are distributed as the target's own.  temperature <= 0.01:
+ * drafts are accepted while they are the row's argmax (the first maximum, as
+ * gbx_select_tokens), the next token is the argmax; uniforms and draft_logits
+ * are not read.  -inf logits are tokens of probability 0.
+ *   n_accepted[b]  drafts accepted
+ *   out_ids[b][.]  n_draft + 1 entries: the accepted drafts, the next token, -1s
+ * A row that gives no distribution (GBX_VERIFY_BAD_ROW) ends its sequence
+ * there with next token -1.  The accepted test sums in fp32 (a draw within
+ * ~1e-6 of the border may go either way); the choice of the next token is
+ * taken in fp64.
+ */
+int gbx_verify_tokens(const float* logits, const float* draft_logits, const int32_t* draft_ids,
+                      const int32_t* draft_len, int64_t B, int n_draft, int vocab, double temperature,
+                      const double* uniforms, int32_t* out_ids, int32_t* n_accepted, int* err_flag,
+                      gbx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
