@@ -78,13 +78,16 @@ def attend(cache, table, kv_len, n_new, q, scale, skip=()):
     """out [B, S, H, hd] in fp64, NaN-filled where no row is computed, and the
     bound on an fp32-grade kernel's error at each entry.
 
-    With A_t = sum_i |q_i k_ti| / scale, the score x_t (in units of log 2)
-    carries the halves' rounding (2^-22 of A), the fp32 sum of hd products
-    (each addition at most 2^-23, truncation included) and a few roundings of
-    |x|; the weight's exponential adds 2^-22 and the rounding of x - m + 14.
-    A weight's own halves, a 64-token sum and the running sums add
-    2^-22 + (64 + L/4 + 40) 2^-23 of sum w |v|.  An error of d in every score
-    moves the output by at most 2 d sum w |v|."""
+    A query enters as 24-bit fixed point: every entry is off by at most qmax 2^-23
+    (half a unit of qmax / 8355711, and the rounding of the product that scales
+    it), so with B_t = qmax sum_i |k_ti| / scale and A_t = sum_i |q_i k_ti| /
+    scale the score x_t (in units of log 2) is off by B 2^-23, plus the fp32
+    joining of three exact sums and its scaling by three factors (8 roundings
+    of at most 2^-24 of A, doubled), plus the rounding of x - max + 23; the
+    weight's exponential adds 2^-22.  A weight is fixed point too, off by half
+    of 2^-23 of its 64-token step's largest (in terms of the step's largest
+    value), and the running sums add (L/4 + 40) 2^-23 of sum w |v|.  An error
+    of d in every score moves the output by at most 2 d sum w |v|."""
     B, S, H, hd = q.shape
     G = H // cache.heads
     out = np.full((B, S, H, hd), np.nan)
@@ -115,8 +118,13 @@ def attend(cache, table, kv_len, n_new, q, scale, skip=()):
                     w /= w.sum()
                     out[b, i, h] = w @ v
                     x2, A2 = np.abs(x) * 1.4427, A * 1.4427
-                    d = (A2 * (2.0 ** -22 + (hd + 8) * 2.0 ** -23) + 6 * 2.0 ** -24 * (x2 + x2.max() + 14)).max() * 0.6932 + 2.0 ** -22
-                    tol[b, i, h] = (2 * d + 2.0 ** -21 + (104 + L / 4) * 2.0 ** -23) * (w @ np.abs(v))
+                    B2 = np.abs(k).sum(1) * np.abs(qq).max() / scale * 1.4427
+                    d = (B2 * 2.0 ** -23 + A2 * 2.0 ** -20 + 6 * 2.0 ** -24 * (x2 + x2.max() + 23)).max() * 0.6932 + 2.0 ** -22
+                    step = pos[see] // 64
+                    top = np.zeros(step.max() + 1)
+                    np.maximum.at(top, step, w)
+                    fixed = top[step].sum() * np.abs(v).max() * 2.0 ** -24
+                    tol[b, i, h] = (2 * d + 2.0 ** -21 + (40 + L / 4) * 2.0 ** -23) * (w @ np.abs(v)) + fixed
     return out, tol
 
 
