@@ -294,6 +294,47 @@ class _KVCacheStruct(ctypes.Structure):
                 ("page", ctypes.c_int32), ("heads", ctypes.c_int32), ("hd", ctypes.c_int32)]
 
 
+class _Torch:
+    """The three things of torch that a cache call needs, looked up once."""
+    int32 = device = stream = None
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.int32 = torch.int32
+        cls.device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else lambda: -1
+        cls.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _device_of(t):
+    """CUDA device index of a tensor, or -1 (an address, a host tensor)."""
+    if _Torch.int32 is None:
+        _Torch.load()
+    d = getattr(t, "device", None)
+    if d is None or d.type != "cuda":
+        return -1
+    return _Torch.device() if d.index is None else d.index
+
+
+def _elsewhere(dev):
+    """Whether `dev` is a GPU other than the current one."""
+    return dev >= 0 and dev != _Torch.device()
+
+
+def _stream_on(dev, stream):
+    """Handle of the stream to launch on: `stream`, or the device's current torch stream."""
+    if stream is None:
+        return _Torch.stream(dev) if dev >= 0 else _stream(None)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _there(dev, fn, *args, **kw):
+    """fn(...) with GPU `dev` current: a kernel runs where its tensors are."""
+    import torch
+    with torch.cuda.device(dev):
+        return fn(*args, **kw)
+
+
 class KVCache:
     """Paged 8-bit key/value cache (gbx_kv_cache): ``KVCache(layers=, pages=,
     heads=, page=, hd=)`` allocates its four tensors on `device`;
@@ -321,36 +362,19 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.layers, self.pages, self.heads, self.page, self.hd = layers, pages, heads, page, hd
         self.device = k.device
+        self._dev = _device_of(k)
         self._c = _KVCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, layers, page,
                                  heads, hd)
         self._ref = ctypes.byref(self._c)
 
 
-def _int32(**tensors):
-    """The index arrays of the cache calls, where they are tensors: int32, contiguous."""
-    for name, t in tensors.items():
-        if t is not None and not isinstance(t, int) and (str(t.dtype) != "torch.int32" or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous int32 tensor")
-
-
-class _on_device:
-    """The launch's device made current: a kernel runs where its tensors are,
-    whichever device the caller has selected."""
-
-    def __init__(self, device):
-        self.guard = None
-        if device is not None and device.type == "cuda":
-            import torch
-            if device.index is not None and device.index != torch.cuda.current_device():
-                self.guard = torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _index(name, t):
+    """Address of an index array: a contiguous int32 tensor, an address or None."""
+    if t is None or isinstance(t, int):
+        return t
+    if t.dtype is not _Torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor")
+    return t.data_ptr()
 
 
 def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_new=None, k_lo=None, v_lo=None,
@@ -358,35 +382,45 @@ def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_
     """Appends row (b, i), i < n_new[b], of k and v (row stride ld) as token
     kv_len[b] - n_new[b] + i of sequence b.  max_pages: the table's row length
     (its last dimension when it is a tensor)."""
-    _int32(table=table, kv_len=kv_len, n_new=n_new)
-    with _on_device(cache.device):
-        _check(lib().gbx_kv_append(cache._ref, layer, _p(table), _max_pages(table, max_pages), _p(kv_len), _p(n_new), B, S,
-                                   _p(k), _p(k_lo), _p(v), _p(v_lo), ld, _p(err_flag), _stream(stream)))
-
-
-def _max_pages(table, max_pages):
-    return table.shape[-1] if max_pages is None else max_pages
+    dev = cache._dev
+    if _elsewhere(dev):
+        return _there(dev, kv_append, cache, layer, k, v, table, kv_len, B=B, S=S, ld=ld, max_pages=max_pages, n_new=n_new,
+                      k_lo=k_lo, v_lo=v_lo, err_flag=err_flag, stream=stream)
+    rc = _lib.gbx_kv_append(cache._ref, layer, _index("table", table), table.shape[-1] if max_pages is None else max_pages,
+                            _index("kv_len", kv_len), _index("n_new", n_new), B, S, _p(k), _p(k_lo), _p(v), _p(v_lo), ld,
+                            _p(err_flag), _stream_on(dev, stream))
+    if rc:
+        _check(rc)
 
 
 def kv_read(cache, layer, table, kv_len, k_out, v_out, *, B, S, ld, max_pages=None, n=None, err_flag=None, stream=None):
     """The fp32 values of each sequence's last n[b] tokens (the mirror of kv_append)."""
-    _int32(table=table, kv_len=kv_len, n=n)
-    with _on_device(cache.device):
-        _check(lib().gbx_kv_read(cache._ref, layer, _p(table), _max_pages(table, max_pages), _p(kv_len), _p(n), B, S,
-                                 _p(k_out), _p(v_out), ld, _p(err_flag), _stream(stream)))
+    dev = cache._dev
+    if _elsewhere(dev):
+        return _there(dev, kv_read, cache, layer, table, kv_len, k_out, v_out, B=B, S=S, ld=ld, max_pages=max_pages, n=n,
+                      err_flag=err_flag, stream=stream)
+    rc = _lib.gbx_kv_read(cache._ref, layer, _index("table", table), table.shape[-1] if max_pages is None else max_pages,
+                          _index("kv_len", kv_len), _index("n", n), B, S, _p(k_out), _p(v_out), ld, _p(err_flag),
+                          _stream_on(dev, stream))
+    if rc:
+        _check(rc)
 
 
 def kv_copy_pages(cache, src, dst, *, n, err_flag=None, stream=None):
     """Page dst[i] becomes page src[i], i < n, in every layer."""
-    _int32(src=src, dst=dst)
-    with _on_device(cache.device):
-        _check(lib().gbx_kv_copy_pages(cache._ref, _p(src), _p(dst), n, _p(err_flag), _stream(stream)))
+    dev = cache._dev
+    if _elsewhere(dev):
+        return _there(dev, kv_copy_pages, cache, src, dst, n=n, err_flag=err_flag, stream=stream)
+    rc = _lib.gbx_kv_copy_pages(cache._ref, _index("src", src), _index("dst", dst), n, _p(err_flag), _stream_on(dev, stream))
+    if rc:
+        _check(rc)
 
 
 def attn_cached_workspace(cache, *, B, S, H, max_pages) -> int:
     """Floats of workspace attn_cached can use for these sizes (0: none)."""
-    with _on_device(cache.device):
-        n = lib().gbx_attn_cached_workspace(cache._ref, B, S, H, max_pages)
+    if _elsewhere(cache._dev):
+        return _there(cache._dev, attn_cached_workspace, cache, B=B, S=S, H=H, max_pages=max_pages)
+    n = _lib.gbx_attn_cached_workspace(cache._ref, B, S, H, max_pages)
     if n < 0:
         _check(-n)
     return n
@@ -395,20 +429,31 @@ def attn_cached_workspace(cache, *, B, S, H, max_pages) -> int:
 def attn_cached(cache, layer, q, out, table, kv_len, *, B, S, H, ld, ld_out, scale, max_pages=None, n_new=None, q_lo=None,
                 out_lo=None, workspace=None, workspace_floats=None, err_flag=None, stream=None):
     """Attention of S rows per sequence over the cached tokens (see gbx.h)."""
-    _int32(table=table, kv_len=kv_len, n_new=n_new)
+    dev = cache._dev
+    if _elsewhere(dev):
+        return _there(dev, attn_cached, cache, layer, q, out, table, kv_len, B=B, S=S, H=H, ld=ld, ld_out=ld_out, scale=scale,
+                      max_pages=max_pages, n_new=n_new, q_lo=q_lo, out_lo=out_lo, workspace=workspace,
+                      workspace_floats=workspace_floats, err_flag=err_flag, stream=stream)
     if workspace_floats is None:
         workspace_floats = workspace.numel() if hasattr(workspace, "numel") else 0
-    with _on_device(cache.device):
-        _check(lib().gbx_attn_cached(cache._ref, layer, _p(q), _p(q_lo), ld, _p(table), _max_pages(table, max_pages),
-                                     _p(kv_len), _p(n_new), B, S, H, scale, _p(out), _p(out_lo), ld_out, _p(workspace),
-                                     workspace_floats, _p(err_flag), _stream(stream)))
+    rc = _lib.gbx_attn_cached(cache._ref, layer, _p(q), _p(q_lo), ld, _index("table", table),
+                              table.shape[-1] if max_pages is None else max_pages, _index("kv_len", kv_len),
+                              _index("n_new", n_new), B, S, H, scale, _p(out), _p(out_lo), ld_out, _p(workspace),
+                              workspace_floats, _p(err_flag), _stream_on(dev, stream))
+    if rc:
+        _check(rc)
 
 
 def verify_tokens(logits, draft_ids, out_ids, n_accepted, *, B, n_draft, vocab, temperature=0.0, uniforms=None,
                   draft_logits=None, draft_len=None, err_flag=None, stream=None):
     """Accepts drafted tokens against the target's logits and picks the next token (see gbx.h)."""
-    _int32(draft_ids=draft_ids, out_ids=out_ids, n_accepted=n_accepted, draft_len=draft_len)
-    with _on_device(getattr(logits, "device", None)):
-        _check(lib().gbx_verify_tokens(_p(logits), _p(draft_logits), _p(draft_ids), _p(draft_len), B, n_draft, vocab,
-                                       float(temperature), _p(uniforms), _p(out_ids), _p(n_accepted), _p(err_flag),
-                                       _stream(stream)))
+    dev = _device_of(logits)
+    if _elsewhere(dev):
+        return _there(dev, verify_tokens, logits, draft_ids, out_ids, n_accepted, B=B, n_draft=n_draft, vocab=vocab,
+                      temperature=temperature, uniforms=uniforms, draft_logits=draft_logits, draft_len=draft_len,
+                      err_flag=err_flag, stream=stream)
+    rc = _lib.gbx_verify_tokens(_p(logits), _p(draft_logits), _index("draft_ids", draft_ids), _index("draft_len", draft_len), B,
+                                n_draft, vocab, temperature, _p(uniforms), _index("out_ids", out_ids),
+                                _index("n_accepted", n_accepted), _p(err_flag), _stream_on(dev, stream))
+    if rc:
+        _check(rc)

@@ -45,6 +45,8 @@
 // Every wait for a copy is bounded (1 s): a warp that gives up stops its
 // steps, waits (bounded) for the copies it has in flight, and its rows come
 // out as NaN with GBX_LINEAR_TIMEOUT in the error flag.
+#include <type_traits>
+
 #include "kv_cache.cuh"
 #include "tcgen05.cuh"
 #include "tf32.cuh"
@@ -53,8 +55,7 @@ namespace gbx {
 
 constexpr int kAcTile = 64;      // tokens per warp and step
 constexpr int kAcMaxCluster = 8;
-constexpr uint32_t kAcMagic = 0x4b400000u;      // 1.5 * 2^23
-constexpr float kAcMagicF = 12582912.0f;
+constexpr float kAcMagicF = 12582912.0f;        // 1.5 * 2^23, bits 0x4b400000
 constexpr float kAcQTop = 8355711.0f;           // 0x7f7f7f: the largest x whose balanced digits fit in 8 bits
 // A weight is 2^(x - max + 23 - 2^-19): just below 2^23 at most, so that adding 2^23
 // leaves it, rounded, in the low 23 bits of the float.
@@ -73,6 +74,7 @@ struct AcArgs {
     int H, G;         // query heads, query heads per key head
     int nrb;          // row blocks per (sequence, key head)
     int nsplit;       // clusters per unit
+    FastDiv by_heads, by_nrb, by_g, by_nsplit, by_hd;
     int vec;          // q rows are 16-byte aligned
     uint64_t first_wait_ns;
 };
@@ -99,13 +101,6 @@ __device__ __forceinline__ void ac_mma(uint32_t (&d)[4], uint32_t a0, uint32_t a
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 
-// 65536 s2 + 256 s1 + s0 of three accumulators that started at kAcMagic.
-__device__ __forceinline__ float ac_join(uint32_t s0, uint32_t s1, uint32_t s2)
-{
-    const float f0 = __uint_as_float(s0) - kAcMagicF, f1 = __uint_as_float(s1) - kAcMagicF, f2 = __uint_as_float(s2) - kAcMagicF;
-    return fmaf(fmaf(f2, 256.0f, f1), 256.0f, f0);
-}
-
 // Digits 0, 1 and 2 of four 24-bit numbers, each digit's four bytes in one word.
 __device__ __forceinline__ void ac_digits(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t& d0, uint32_t& d1, uint32_t& d2)
 {
@@ -122,6 +117,46 @@ __device__ __forceinline__ uint4 ac_lds(uint32_t at)
     return v;
 }
 
+// Constants that instructions take from registers: the accumulators' start, the
+// zero digits, and pairs for the packed fp32 instructions.  Opaque, so that the
+// compiler holds them in registers of their own instead of setting them up
+// before every use.
+struct AcConst {
+    uint32_t c[4], z[2];
+    float2 less, by, two23;
+    __device__ __forceinline__ static float reg(float x)
+    {
+        float y;
+        asm volatile("mov.f32 %0, %1;" : "=f"(y) : "f"(x));
+        return y;
+    }
+    __device__ __forceinline__ AcConst()
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("mov.u32 %0, 0x4b400000;" : "=r"(c[i]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) asm volatile("mov.u32 %0, 0;" : "=r"(z[i]));
+        less = make_float2(reg(-kAcMagicF), reg(-kAcMagicF));
+        by = make_float2(reg(256.0f), reg(256.0f));
+        two23 = make_float2(reg(8388608.0f), reg(8388608.0f));
+    }
+};
+
+// 65536 s2 + 256 s1 + s0 of accumulators that started at 0x4b400000, two
+// neighbouring columns at a time (packed fp32, two lanes an instruction).
+__device__ __forceinline__ float2 ac_join(uint32_t s0, uint32_t t0, uint32_t s1, uint32_t t1, uint32_t s2, uint32_t t2, const AcConst& k)
+{
+    const float2 f0 = __fadd2_rn(make_float2(__uint_as_float(s0), __uint_as_float(t0)), k.less);
+    const float2 f1 = __fadd2_rn(make_float2(__uint_as_float(s1), __uint_as_float(t1)), k.less);
+    const float2 f2 = __fadd2_rn(make_float2(__uint_as_float(s2), __uint_as_float(t2)), k.less);
+    return __ffma2_rn(__ffma2_rn(f2, k.by, f1), k.by, f0);
+}
+
+// 32-column blocks of a head, in pairs: a lane's 16 key bytes feed two.
+constexpr int ac_chunks(int hd) { return hd > 64 ? 4 : 2; }
+// Bytes between the 16-token groups of a slot.
+constexpr int ac_pitch(int hd) { return 16 * hd + 32; }
+
 // Digits of RT tiles of 8 rows.  d0, d1: [rt][m][2] (the two A registers of an
 // 8-token or 8-column half), d2 likewise.
 template <int RT, int M>
@@ -129,29 +164,28 @@ struct AcDigits {
     uint32_t d0[RT][M][2], d1[RT][M][2], d2[RT][M][2];
 };
 
-// s[rt][0..3 rows' sums]: one n8 column group against one 16-byte word group.
+// s[rt]: this lane's row of tile rt against its two columns of one n8 group,
+// whose B operands are the 16 bytes b[0], b[1], ..
 template <bool U, int RT, int M>
-__device__ __forceinline__ void ac_dot(float (&s)[RT][2], const AcDigits<RT, M>& a, int m0, int mn, const uint4* b)
+__device__ __forceinline__ void ac_dot(float2 (&s)[RT], const AcDigits<RT, M>& a, const uint4* b, const AcConst& k)
 {
     uint32_t x[RT][4], y[4];
 #pragma unroll
-    for (int m = 0; m < mn; ++m) {
+    for (int m = 0; m < M; ++m) {
         const uint4 w = b[m >> 1];
         const uint32_t b0 = m & 1 ? w.z : w.x, b1 = m & 1 ? w.w : w.y;
-        const int q = m0 + m;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            if (m == 0) ac_mma<U>(x[rt], a.d0[rt][q][0], a.d1[rt][q][0], a.d0[rt][q][1], a.d1[rt][q][1], b0, b1, kAcMagic, kAcMagic, kAcMagic, kAcMagic);
-            else ac_mma<U>(x[rt], a.d0[rt][q][0], a.d1[rt][q][0], a.d0[rt][q][1], a.d1[rt][q][1], b0, b1, x[rt][0], x[rt][1], x[rt][2], x[rt][3]);
+            if (m == 0) ac_mma<U>(x[rt], a.d0[rt][m][0], a.d1[rt][m][0], a.d0[rt][m][1], a.d1[rt][m][1], b0, b1, k.c[0], k.c[1], k.c[2], k.c[3]);
+            else ac_mma<U>(x[rt], a.d0[rt][m][0], a.d1[rt][m][0], a.d0[rt][m][1], a.d1[rt][m][1], b0, b1, x[rt][0], x[rt][1], x[rt][2], x[rt][3]);
         }
-        const uint32_t z0 = RT == 2 ? a.d2[RT - 1][q][0] : 0u, z1 = RT == 2 ? a.d2[RT - 1][q][1] : 0u;
-        if (m == 0) ac_mma<U>(y, a.d2[0][q][0], z0, a.d2[0][q][1], z1, b0, b1, kAcMagic, kAcMagic, kAcMagic, kAcMagic);
-        else ac_mma<U>(y, a.d2[0][q][0], z0, a.d2[0][q][1], z1, b0, b1, y[0], y[1], y[2], y[3]);
+        const uint32_t z0 = RT == 2 ? a.d2[RT - 1][m][0] : k.z[0], z1 = RT == 2 ? a.d2[RT - 1][m][1] : k.z[1];
+        if (m == 0) ac_mma<U>(y, a.d2[0][m][0], z0, a.d2[0][m][1], z1, b0, b1, k.c[0], k.c[1], k.c[2], k.c[3]);
+        else ac_mma<U>(y, a.d2[0][m][0], z0, a.d2[0][m][1], z1, b0, b1, y[0], y[1], y[2], y[3]);
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        s[rt][0] = ac_join(x[rt][0], x[rt][2], y[2 * rt]);
-        s[rt][1] = ac_join(x[rt][1], x[rt][3], y[2 * rt + 1]);
+        s[rt] = ac_join(x[rt][0], x[rt][1], x[rt][2], x[rt][3], y[2 * rt], y[2 * rt + 1], k);
     }
 }
 
@@ -162,14 +196,14 @@ struct AcUnit {
     KvSeq seq;
 };
 
-__device__ __forceinline__ AcUnit ac_unit(const AcArgs& a, int64_t unit, int R, bool* bad_len)
+__device__ __forceinline__ AcUnit ac_unit(const AcArgs& a, uint32_t unit, int R, bool* bad_len)
 {
     AcUnit u;
-    u.h = (int)(unit % a.c.heads);
-    const int64_t w = unit / a.c.heads;
-    u.b = (int)(w / a.nrb);
+    const uint32_t w = fast_div(unit, a.by_heads);
+    u.h = (int)(unit - w * a.c.heads);
+    u.b = (int)fast_div(w, a.by_nrb);
     u.seq = kv_seq(a.c, u.b, bad_len);
-    u.r0 = (int)(w % a.nrb) * R;
+    u.r0 = (int)(w - u.b * a.nrb) * R;
     u.rows = min(R, u.seq.n * a.G - u.r0);   // valid rows of this block, if positive
     return u;
 }
@@ -177,7 +211,7 @@ __device__ __forceinline__ AcUnit ac_unit(const AcArgs& a, int64_t unit, int R, 
 // Where row r of the unit lies in q or out, but for the column.
 __device__ __forceinline__ int64_t ac_row(const AcArgs& a, const AcUnit& u, int r, int64_t ld)
 {
-    const int rr = u.r0 + r, i = rr / a.G;
+    const int rr = u.r0 + r, i = (int)fast_div(rr, a.by_g);
     return ((int64_t)u.b * a.c.S + i) * ld + (int64_t)(u.h * a.G + rr - i * a.G) * a.c.hd;
 }
 
@@ -195,15 +229,16 @@ __device__ __forceinline__ void ac_store(const AcArgs& a, int64_t at, float v)
 
 // The query digits of rows base + 8 rt + n of the unit, the factor qs that turns
 // a code sum into log2(e) q.c / scale, and the keys each row sees.
-template <int NCH, int RT>
-__device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int base, AcDigits<RT, 2 * NCH>& q, float (&qs)[RT], int (&limit)[RT])
+template <int HD, int RT>
+__device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int base, AcDigits<RT, ac_chunks(HD)>& q, float (&qs)[RT], int (&limit)[RT])
 {
-    const int lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3, hd = a.c.hd;
+    constexpr int NCH = ac_chunks(HD) / 2;
+    const int lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int r = base + 8 * rt + n;
         const bool ok = r < u.rows;
-        limit[rt] = ok ? u.seq.len - u.seq.n + (u.r0 + r) / a.G + 1 : 0;
+        limit[rt] = ok ? u.seq.len - u.seq.n + (int)fast_div(u.r0 + r, a.by_g) + 1 : 0;
         const int64_t at = ac_row(a, u, r, a.ld);
         float x[NCH][16];
         float big = 0.0f, bad = 0.0f;
@@ -213,7 +248,7 @@ __device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (ok && col < hd) {
+                if (ok && col < HD) {
                     const float* p = a.q_hi + at + col + e;
                     const float* pl = a.q_lo ? a.q_lo + at + col + e : nullptr;
                     if (a.vec) {
@@ -264,31 +299,30 @@ __device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int
     }
 }
 
-// One step: 64 tokens from t0 in shared memory (kb: keys, vb: values; groups
-// `pitch` bytes apart) against RT tiles of 8 rows.  ks, vs: the scales of group
+// One step, first half: the scores of 64 tokens whose keys lie at kb (groups
+// `pitch` bytes apart), the running maximum and sum, and the weights' digits.  ks, vs: the scales of group
 // cc; seen: that group can be read.  edge: some valid
 // row does not see all 64 (rows past the unit's end hold zero queries and are never stored).
-template <int NCH, int RT>
-__device__ __forceinline__ void ac_step(uint32_t kb, uint32_t vb, int pitch, int hd, int t0, bool seen, bool edge, float ks, float vs,
-                                        const AcDigits<RT, 2 * NCH>& q, const float (&qs)[RT], const int (&limit)[RT],
-                                        float (&m)[RT], float (&l)[RT], float (&o)[RT][8 * NCH][2])
+template <int HD, int RT>
+__device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool edge, float ks, float vs,
+                                          const AcDigits<RT, ac_chunks(HD)>& q, const float (&qs)[RT], const int (&limit)[RT],
+                                          float (&m)[RT], float (&l)[RT], AcDigits<RT, 2>& p, float (&alpha)[RT], float (&beta)[RT],
+                                          const AcConst& kc)
 {
     const int lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
-    float s[RT][8][2];
+    constexpr int NCH = ac_chunks(HD) / 2, pitch = ac_pitch(HD);
+    float2 s[RT][8];
     // key side: this lane's tokens are 2g + (n & 1) of group n / 2
-    const uint32_t kp = kb + (n >> 1) * pitch + (n & 1) * hd + 16 * cc;
+    const uint32_t kp = kb + (n >> 1) * pitch + (n & 1) * HD + 16 * cc;
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
         uint4 w[NCH];
 #pragma unroll
-        for (int ch = 0; ch < NCH; ++ch) w[ch] = ac_lds(kp + 2 * g * hd + 64 * ch);
-        float d[RT][2];
-        ac_dot<false, RT, 2 * NCH>(d, q, 0, 2 * NCH, w);
+        for (int ch = 0; ch < NCH; ++ch) w[ch] = ac_lds(kp + 2 * g * HD + 64 * ch);
+        float2 d[RT];
+        ac_dot<false, RT, ac_chunks(HD)>(d, q, w, kc);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            s[rt][g][0] = d[rt][0];
-            s[rt][g][1] = d[rt][1];
-        }
+        for (int rt = 0; rt < RT; ++rt) s[rt][g] = d[rt];
     }
     // the step's largest value scale; a NaN scale stays in the ratio, where
     // only the rows that see its group meet it
@@ -296,198 +330,225 @@ __device__ __forceinline__ void ac_step(uint32_t kb, uint32_t vb, int pitch, int
     vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
     const float vr = vmax > 0.0f ? __fdividef(vs, vmax) : (vs == vs ? 0.0f : vs);
     vmax = vmax > 0.0f ? vmax : 0.0f;
-    AcDigits<RT, 2> p;
-    float alpha[RT], beta[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float f = qs[rt] * ks;
+        const float2 f = splat2(qs[rt] * ks);
         float mt = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                s[rt][g][e] *= f;
-                if (edge && !(seen && t0 + 16 * cc + 2 * g + e < limit[rt])) s[rt][g][e] = -INFINITY;
-                mt = fmaxf(mt, s[rt][g][e]);
+        for (int g = 0; g < 8; ++g) {
+            s[rt][g] = __fmul2_rn(s[rt][g], f);
+            if (edge) {
+                const int t = t0 + 16 * cc + 2 * g;
+                if (!seen || t >= limit[rt]) s[rt][g].x = -INFINITY;
+                if (!seen || t + 1 >= limit[rt]) s[rt][g].y = -INFINITY;
             }
+            mt = fmaxf(fmaxf(mt, s[rt][g].x), s[rt][g].y);
+        }
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
         const float mx = fmaxf(m[rt], mt), base = mx == -INFINITY ? 0.0f : mx;
         alpha[rt] = ac_exp2(m[rt] - base);
         beta[rt] = ac_exp2(mt - base);
         m[rt] = mx;
-        const float sub = mt == -INFINITY ? 0.0f : kAcPOff - mt;
+        const float2 sub = splat2(mt == -INFINITY ? 0.0f : kAcPOff - mt);
         const float vrr = !edge || t0 + 16 * cc < limit[rt] ? vr : 0.0f;
-        float sum = 0.0f;
-        uint32_t y[8][2];
+        float2 sum = make_float2(0.0f, 0.0f), y[8];
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float x = ac_exp2(s[rt][g][e] + sub);
-                sum += x;
-                y[g][e] = __float_as_uint(fmaf(x, vrr, 8388608.0f));
-            }
-        sum = fmaf(vrr, 0.0f, sum);   // a NaN scale: its digits above are no numbers, the sum says so
-        l[rt] = fmaf(l[rt], alpha[rt], sum * beta[rt]);
+        for (int g = 0; g < 8; ++g) {
+            float2 x = __fadd2_rn(s[rt][g], sub);
+            x = make_float2(ac_exp2(x.x), ac_exp2(x.y));
+            sum = __fadd2_rn(sum, x);
+            y[g] = __ffma2_rn(x, splat2(vrr), kc.two23);
+        }
+        // a NaN scale: its digits are no numbers, the sum says so
+        l[rt] = fmaf(l[rt], alpha[rt], fmaf(vrr, 0.0f, sum.x + sum.y) * beta[rt]);
         beta[rt] *= vmax;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-            ac_digits(y[2 * w][0], y[2 * w][1], y[2 * w + 1][0], y[2 * w + 1][1], p.d0[rt][w >> 1][w & 1], p.d1[rt][w >> 1][w & 1],
-                      p.d2[rt][w >> 1][w & 1]);
-    }
-    const uint32_t vp = vb + cc * pitch + n * 16;
-#pragma unroll
-    for (int j = 0; j < 8 * NCH; ++j) {
-        if (8 * j >= hd) break;
-        const uint4 w = ac_lds(vp + 8 * j * 16);
-        float d[RT][2];
-        ac_dot<true, RT, 2>(d, p, 0, 2, &w);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            o[rt][j][0] = fmaf(o[rt][j][0], alpha[rt], d[rt][0] * beta[rt]);
-            o[rt][j][1] = fmaf(o[rt][j][1], alpha[rt], d[rt][1] * beta[rt]);
-        }
+            ac_digits(__float_as_uint(y[2 * w].x), __float_as_uint(y[2 * w].y), __float_as_uint(y[2 * w + 1].x),
+                      __float_as_uint(y[2 * w + 1].y), p.d0[rt][w >> 1][w & 1], p.d1[rt][w >> 1][w & 1], p.d2[rt][w >> 1][w & 1]);
     }
 }
 
-// NCH: 64-column chunks of the head; RT: 8-row tiles; W: warps; NS: ring stages.
-template <int NCH, int RT, int W, int NS>
+// Second half: the output rows, rescaled by alpha, with the 64 tokens' values at
+// vb added (beta: what a sum of digits and codes stands for).
+template <int HD, int RT>
+__device__ __forceinline__ void ac_values(uint32_t vb, const AcDigits<RT, 2>& p, const float (&alpha)[RT],
+                                          const float (&beta)[RT], float2 (&o)[RT][HD / 8], const AcConst& kc)
+{
+    const int lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
+    const uint32_t vp = vb + cc * ac_pitch(HD) + n * 16;
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) {
+        const uint4 w = ac_lds(vp + 8 * j * 16);
+        float2 d[RT];
+        ac_dot<true, RT, 2>(d, p, &w, kc);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][j] = __ffma2_rn(o[rt][j], splat2(alpha[rt]), __fmul2_rn(d[rt], splat2(beta[rt])));
+    }
+}
+
+// HD: head width; RT: 8-row tiles; W: warps; NS: slots of a warp's ring, each
+// the keys or the values of one step.
+template <int HD, int RT, int W, int NS>
 __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
 {
     grid_dependency_wait();
     constexpr int R = 8 * RT, T = 32 * W;
     extern __shared__ __align__(128) uint8_t ac_smem[];
     __shared__ uint64_t bars[W][NS];
-    __shared__ float s_scale[W][NS][2][4];
+    __shared__ float s_scale[W][4][2][4];   // of step t in [t & 3]: key and value scales of the four groups
     __shared__ int s_abort;
     const KvLayer& c = a.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
     uint32_t rank, csize;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
-    const int64_t cid = blockIdx.x / csize;
-    const int split = (int)(cid % a.nsplit);
-    const int64_t unit = cid / a.nsplit;
+    const uint32_t cid = blockIdx.x >> (31 - __clz((int)csize));   // csize is a power of two
+    const uint32_t unit = fast_div(cid, a.by_nsplit);
+    const int split = (int)(cid - unit * a.nsplit);
     bool bad_len;
     const AcUnit u = ac_unit(a, unit, R, &bad_len);
     if (bad_len && threadIdx.x == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
     if (u.rows <= 0) return;   // every CTA of the cluster alike
-    const int hd = c.hd;
+    constexpr int hd = HD;
 
     // ---------------------------------------------------- this warp's ring
-    // a stage: 4 key groups, 4 value groups, each 16 hd bytes and 32 of padding
-    // (the four groups' same columns then lie in different banks)
-    const int pitch = 16 * hd + 32, stage = 8 * pitch;
-    const uint32_t ring = tc::smem_u32(ac_smem) + warp * NS * stage;
+    // A slot: four groups of 16 hd bytes and 32 of padding (the groups' same
+    // columns then lie in different banks).  Operation 2k is the keys of this
+    // warp's k-th step, 2k + 1 its values; operation j uses slot j mod NS and
+    // is started as soon as operation j - NS has been read.
+    constexpr int pitch = ac_pitch(HD), slot_bytes = 4 * pitch;
+    const uint32_t ring = tc::smem_u32(ac_smem) + warp * NS * slot_bytes;
     const uint32_t bar0 = tc::smem_u32(&bars[warp][0]);
     if (lane == 0) {
-        for (int s = 0; s < NS; ++s) tc::mbar_init(bar0 + 8 * s, 1);
+        for (int s = 0; s < NS; ++s) tc::mbar_init(bar0 + 8 * s, 9);
         tc::fence_mbar_init();
     }
     if (threadIdx.x == 0) s_abort = 0;
     __syncthreads();
-    const int maxlim = u.seq.len - u.seq.n + (u.r0 + u.rows - 1) / a.G + 1;   // keys the last row sees
-    const int minlim = u.seq.len - u.seq.n + u.r0 / a.G + 1;                  // and the first
+    const int maxlim = u.seq.len - u.seq.n + (int)fast_div(u.r0 + u.rows - 1, a.by_g) + 1;   // keys the last row sees
+    const int minlim = u.seq.len - u.seq.n + (int)fast_div(u.r0, a.by_g) + 1;                // and the first
     const int steps = (maxlim + kAcTile - 1) / kAcTile;
     const int stride = (int)csize * a.nsplit * W;
     const int first = (split * (int)csize + (int)rank) * W + warp;
     const int lg16 = c.log_page - 4;
     const int64_t page_bytes = (int64_t)hd << c.log_page;
-    // the page of this lane's group (lane & 3) of a step: -2 past the last key
+    // the page of this lane's group (lane & 3) of a step; -1: not in the pool, -2: past the last key
     auto look = [&](int step) {
         const int g = 4 * step + cc;
         return step < steps && 16 * g < maxlim ? kv_page(c, u.b, g >> lg16) : -2;
     };
-    // starts a step's copies into stage s; lanes 0-3 the keys, 4-7 the values
-    auto issue = [&](int step, int s, int page) {
-        const unsigned valid = __ballot_sync(0xffffffffu, page >= 0) & 0xffu;
-        if (lane == 0) tc::mbar_arrive_expect_tx(bar0 + 8 * s, (uint32_t)__popc(valid) * 16u * (uint32_t)hd);
+    // Starts the copies of this warp's k-th step's keys (which = 0) or values
+    // into slot s, and with the keys those of the groups' scales, -0 standing
+    // for the scales of a group that cannot be read.  A slot's phase is lane
+    // 0's arrival with the byte count and one of each of lanes 0-7.
+    auto issue = [&](int which, int k, int s, int page) {
+        const uint32_t bar = bar0 + 8 * s;
+        const unsigned valid = __ballot_sync(0xffffffffu, page >= 0) & 0xfu;
+        if (lane == 0) tc::mbar_arrive_expect_tx(bar, (uint32_t)__popc(valid) * 16u * (uint32_t)hd);
         __syncwarp();
-        if (lane < 8 && page >= 0) {
-            const int g = 4 * step + cc;
-            const int8_t* src = (lane < 4 ? c.k : c.v) + ((int64_t)page * c.heads + u.h) * page_bytes + (g & ((1 << lg16) - 1)) * 16 * hd;
-            tc::bulk_load(ring + s * stage + lane * pitch, src, 16u * hd, bar0 + 8 * s);
+        if (lane < 8) {
+            const int g = 4 * (first + k * stride) + cc;
+            const int64_t ph = (int64_t)page * c.heads + u.h;
+            if (lane < 4 && page >= 0)
+                tc::bulk_load(ring + s * slot_bytes + lane * pitch,
+                              (which ? c.v : c.k) + ph * page_bytes + (g & ((1 << lg16) - 1)) * 16 * hd, 16u * hd, bar);
+            float* to = &s_scale[warp][k & 3][lane >> 2][cc];
+            if (which == 0 && page >= 0) {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(to)), "l"((lane < 4 ? c.ks : c.vs) + ph) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+            } else {
+                if (which == 0) *to = -0.0f;
+                tc::mbar_arrive(bar);
+            }
+            if (which == 0 && page == -1 && lane < 4) kv_flag(c.err, GBX_KV_BAD_PAGE);
         }
-        if (page == -1 && lane < 4) kv_flag(c.err, GBX_KV_BAD_PAGE);
-    };
-    // lane 0-3: key scale of group cc, 4-7: value scale; NaN-free 0 where there is no page.
-    // The sign of a zero says whether the group can be read.
-    auto scale_of = [&](int page) {
-        if (page < 0) return -0.0f;
-        return (lane < 4 ? c.ks : c.vs)[(int64_t)page * c.heads + u.h];
     };
 
-    int pg = look(first);
-    float sc = 0.0f;
-    int issued = 0;      // steps whose copies this warp has started
-    constexpr int D = NS - 1;
+    // pages of steps k + 1 and k + 2 of this warp while it works on step k
+    static_assert(NS == 3 || NS == 4, "the page look-ahead below is two steps");
+    int pg[3];
 #pragma unroll
-    for (int k = 0; k < D; ++k) {
-        const int step = first + k * stride;
-        if (step < steps) {
-            issue(step, k, pg);
-            sc = scale_of(pg);
-            pg = look(step + stride);
-            if (lane < 8) s_scale[warp][k][lane >> 2][cc] = sc;
+    for (int k = 0; k < 3; ++k) pg[k] = look(first + k * stride);
+    int issued = 0, read = 0;   // operations
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+        if (first + (j >> 1) * stride < steps) {
+            issue(j & 1, j >> 1, j, pg[j >> 1]);
             ++issued;
         }
-    }
-    __syncwarp();
 
-    AcDigits<RT, 2 * NCH> q;
+    AcDigits<RT, ac_chunks(HD)> q;
     float qs[RT];
     int limit[RT];
-    ac_queries<NCH, RT>(a, u, 0, q, qs, limit);
+    ac_queries<HD, RT>(a, u, 0, q, qs, limit);
 
-    float o[RT][8 * NCH][2];
+    float2 o[RT][HD / 8];
     float m[RT], l[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         m[rt] = -INFINITY;
         l[rt] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8 * NCH; ++j) o[rt][j][0] = o[rt][j][1] = 0.0f;
+        for (int j = 0; j < HD / 8; ++j) o[rt][j] = make_float2(0.0f, 0.0f);
     }
 
+    const AcConst kc;
     bool dead = false;
-    int done = 0, st = 0, last_put = -1;
+    int slot = 0;            // of the next operation to be read
     uint32_t phase = 0;
     volatile int* abort = &s_abort;
-    for (int step = first; step < steps; step += stride, ++done) {
-        if (last_put >= 0 && lane < 8) s_scale[warp][last_put][lane >> 2][cc] = sc;
-        __syncwarp();   // and every lane has read the stage that is filled next
-        last_put = -1;
-        const int ahead = step + D * stride;
-        if (ahead < steps) {
-            const int s = st + D >= NS ? st + D - NS : st + D;
-            issue(ahead, s, pg);
-            sc = scale_of(pg);
-            pg = look(ahead + stride);
-            last_put = s;
-            ++issued;
+    uint64_t limit_ns = a.first_wait_ns;
+    auto next_slot = [&] {
+        ++read;
+        if (++slot == NS) {
+            slot = 0;
+            phase ^= 1;
         }
-        const uint64_t limit_ns = done == 0 ? a.first_wait_ns : kDeviceWaitNs;
-        if (limit_ns == 0 || !tc::mbar_wait(bar0 + 8 * st, phase, abort, limit_ns)) {
+    };
+    int k = 0;
+    for (int step = first; step < steps; step += stride, ++k) {
+        if (limit_ns == 0 || !tc::mbar_wait(bar0 + 8 * slot, phase, abort, limit_ns)) {
             dead = true;
             break;
         }
-        const float ks = s_scale[warp][st][0][cc], vs = s_scale[warp][st][1][cc];
+        limit_ns = kDeviceWaitNs;
+        const float ks = s_scale[warp][k & 3][0][cc], vs = s_scale[warp][k & 3][1][cc];
         const bool seen = !(ks == 0.0f && signbit(ks));
         const int t0 = step * kAcTile;
         const bool edge = __any_sync(0xffffffffu, !seen) || t0 + kAcTile > minlim;
-        const uint32_t kb = ring + st * stage;
-        if (edge) ac_step<NCH, RT>(kb, kb + 4 * pitch, pitch, hd, t0, seen, true, ks, vs, q, qs, limit, m, l, o);
-        else ac_step<NCH, RT>(kb, kb + 4 * pitch, pitch, hd, t0, true, false, ks, vs, q, qs, limit, m, l, o);
-        if (++st == NS) {
-            st = 0;
-            phase ^= 1;
+        AcDigits<RT, 2> p;
+        float alpha[RT], beta[RT];
+        const uint32_t kb = ring + slot * slot_bytes;
+        if (edge) ac_scores<HD, RT>(kb, t0, seen, true, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+        else ac_scores<HD, RT>(kb, t0, true, false, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+        // the keys have been read: operation 2k + NS
+        __syncwarp();
+        if (NS == 3 ? step + stride < steps : step + 2 * stride < steps) {
+            issue(NS == 3, k + (NS == 3 ? 1 : 2), slot, pg[NS == 3 ? 1 : 2]);
+            ++issued;
         }
+        next_slot();
+        if (!tc::mbar_wait(bar0 + 8 * slot, phase, abort, kDeviceWaitNs)) {
+            dead = true;
+            break;
+        }
+        ac_values<HD, RT>(ring + slot * slot_bytes, p, alpha, beta, o, kc);
+        // the values have been read: operation 2k + 1 + NS
+        __syncwarp();
+        if (step + 2 * stride < steps) {
+            issue(NS != 3, k + 2, slot, pg[2]);
+            ++issued;
+        }
+        next_slot();
+        pg[1] = pg[2];
+        pg[2] = look(step + 3 * stride);
     }
     if (dead) {
         // the copies in flight land before anything else happens to this memory
         *abort = 1;
-        for (int k = done; k < issued; ++k) tc::mbar_wait(bar0 + 8 * (k % NS), (k / NS) & 1, nullptr, kDeviceWaitNs);
+        for (int j = read; j < issued; ++j) tc::mbar_wait(bar0 + 8 * (j % NS), (j / NS) & 1, nullptr, kDeviceWaitNs);
         if (lane == 0) kv_flag(c.err, GBX_LINEAR_TIMEOUT);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) l[rt] = __int_as_float(0x7fc00000);
@@ -510,15 +571,14 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
                 s_l[warp * R + r] = l[rt];
             }
 #pragma unroll
-            for (int j = 0; j < 8 * NCH; ++j)
-                if (8 * j < hd)
-                    *reinterpret_cast<float2*>(s_o + (warp * R + r) * hd + 8 * j + 2 * cc) = make_float2(o[rt][j][0], o[rt][j][1]);
+            for (int j = 0; j < HD / 8; ++j)
+                *reinterpret_cast<float2*>(s_o + (warp * R + r) * hd + 8 * j + 2 * cc) = o[rt][j];
         }
     }
     __syncthreads();
     const bool alone = csize == 1 && a.nsplit == 1;
     for (int e = threadIdx.x; e < nr * hd; e += T) {
-        const int r = e / hd, col = e - r * hd;
+        const int r = e / HD, col = e - r * HD;
         float mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w * R + r]);
@@ -549,7 +609,7 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
         return v;
     };
     for (int e = (int)rank * T + threadIdx.x; e < nr * hd; e += (int)csize * T) {
-        const int r = e / hd, col = e - r * hd;
+        const int r = e / HD, col = e - r * HD;
         float mx = -INFINITY;
         for (uint32_t p = 0; p < csize; ++p) mx = fmaxf(mx, peer(p, s_m + W * R + r));
         const float base = mx == -INFINITY ? 0.0f : mx;
@@ -562,7 +622,7 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
         if (a.nsplit == 1) {
             ac_store(a, ac_row(a, u, r, a.ld_out) + col, ll == 0.0f ? 0.0f : acc / ll);
         } else {
-            float* w = a.ws + (unit * a.nsplit + split) * (int64_t)(R * (hd + 2));
+            float* w = a.ws + ((int64_t)unit * a.nsplit + split) * (R * (hd + 2));
             w[r * hd + col] = acc;
             if (col == 0) {
                 w[R * hd + r] = mx;
@@ -577,14 +637,14 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
 __global__ void __launch_bounds__(256) attn_cached_join_kernel(const AcArgs a, int R)
 {
     grid_dependency_wait();
-    const int64_t unit = blockIdx.x;
+    const uint32_t unit = blockIdx.x;
     bool bad_len;
     const AcUnit u = ac_unit(a, unit, R, &bad_len);
     const int hd = a.c.hd;
     const int64_t part = (int64_t)R * (hd + 2);
     for (int e = threadIdx.x; e < u.rows * hd; e += 256) {
-        const int r = e / hd, col = e - r * hd;
-        const float* w = a.ws + unit * a.nsplit * part;
+        const int r = (int)fast_div(e, a.by_hd), col = e - r * hd;
+        const float* w = a.ws + (int64_t)unit * a.nsplit * part;
         float mx = -INFINITY;
         for (int p = 0; p < a.nsplit; ++p) mx = fmaxf(mx, w[p * part + R * hd + r]);
         const float base = mx == -INFINITY ? 0.0f : mx;
@@ -600,11 +660,16 @@ __global__ void __launch_bounds__(256) attn_cached_join_kernel(const AcArgs a, i
 }
 
 // ---------------------------------------------------------------- launch
-// Warps per CTA and ring stages: about 100 KB of ring, two CTAs to an SM.
-constexpr int kAcW1 = 4, kAcS1 = 3, kAcW2 = 3, kAcS2 = 2;
+// Warps per CTA and ring slots.  Measured at 256 sequences x 25 heads x 2048 tokens
+// of width 64: 256 us with 4 warps and 3 slots (4 CTAs to an SM), 257 with 2 and 3,
+// 275 with 2 and 4, 290 with 4 and 4, 339 with 1 and 4; at 2 x 8 heads x 120,001
+// tokens of width 128: 93 with 4 and 3, 101 with 3 and 3, 103 with 2 and 3.
+constexpr int kAcWarps = 4, kAcSlots = 3;
+
+constexpr int kAcSmemPerSM = 228 * 1024;
 
 struct AcPlan {
-    int rt, nch, nrb, csize, nsplit;
+    int rt, nrb, csize, nsplit;
     int64_t units, ws_floats;
 };
 
@@ -614,33 +679,46 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, Ac
     if (device_info(&di) != GBX_OK) return GBX_ECUDA;
     const int G = H / c->heads;
     const int64_t rows = (int64_t)S * G;
-    p->nch = c->hd > 64 ? 2 : 1;
     p->rt = rows > 8 ? 2 : 1;
-    const int R = 8 * p->rt, W = p->nch == 1 ? kAcW1 : kAcW2;
+    const int R = 8 * p->rt, W = kAcWarps, NS = kAcSlots;
     const int64_t nrb = (rows + R - 1) / R;
     p->units = (int64_t)B * c->heads * nrb;
     if (nrb > 0x7fffffff || p->units * kAcMaxCluster > 0x7fffffffLL)
         return set_error(GBX_ERANGE, "gbx_attn_cached: B=%d S=%d H=%d too large", B, S, H);
     p->nrb = (int)nrb;
-    // two CTAs per SM; a warp has a step to itself at least
+    // The CTAs that share a unit: as many as keep every CTA resident at once (a
+    // second, partly filled wave costs more than the longer loops), a step at
+    // least to every warp.  Within a cluster they meet on the chip; beyond 8 in
+    // the workspace, which costs a second launch and is taken where it at least
+    // doubles the CTAs.
     const int64_t steps = ((int64_t)max_pages * c->page + kAcTile - 1) / kAcTile;
-    const int64_t want = 2 * (int64_t)di.sm_count;
+    const int64_t resident = (int64_t)di.sm_count * (int64_t)((size_t)kAcSmemPerSM / (W * NS * 4 * ac_pitch(c->hd) + 2048));
+    int64_t share = resident / p->units;
+    if (share > (steps + W - 1) / W) share = (steps + W - 1) / W;
     p->csize = 1;
-    while (p->csize < kAcMaxCluster && p->units * p->csize < want && (int64_t)p->csize * W < steps) p->csize *= 2;
     p->nsplit = 1;
-    if (p->csize == kAcMaxCluster)
-        while (p->nsplit < 64 && p->units * p->csize * p->nsplit < want && (int64_t)p->nsplit * p->csize * W * 4 < steps)
-            p->nsplit *= 2;
+    while (p->csize < kAcMaxCluster && 2 * p->csize <= share) p->csize *= 2;
+    if (share >= 2 * kAcMaxCluster) {
+        int64_t best = 0;
+        for (int cs = kAcMaxCluster; cs >= 1; cs /= 2) {
+            const int64_t ns = share / cs > 64 ? 64 : share / cs;
+            if (cs * ns > best) {
+                best = cs * ns;
+                p->csize = cs;
+                p->nsplit = (int)ns;
+            }
+        }
+    }
     p->ws_floats = p->nsplit > 1 ? p->units * p->nsplit * R * (c->hd + 2) : 0;
     return GBX_OK;
 }
 
-template <int NCH, int RT, int W, int NS>
+template <int HD, int RT>
 static int ac_launch(const AcArgs& a, const AcPlan& p, cudaStream_t s)
 {
-    auto k = attn_cached_kernel<NCH, RT, W, NS>;
-    constexpr int R = 8 * RT;
-    const size_t ring = (size_t)W * NS * 8 * (16 * a.c.hd + 32);
+    constexpr int R = 8 * RT, W = kAcWarps, NS = kAcSlots;
+    auto k = attn_cached_kernel<HD, RT, W, NS>;
+    const size_t ring = (size_t)W * NS * 4 * ac_pitch(HD);
     const size_t meet = sizeof(float) * (size_t)(W + 1) * R * (a.c.hd + 2);
     const size_t smem = ring > meet ? ring : meet;
     if (smem > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
@@ -725,10 +803,26 @@ extern "C" int gbx_attn_cached(const gbx_kv_cache* cache_host, int layer, const 
     a.G = H / a.c.heads;
     a.nrb = p.nrb;
     a.nsplit = p.nsplit;
+    a.by_heads = make_fastdiv(a.c.heads);
+    a.by_nrb = make_fastdiv(p.nrb);
+    a.by_g = make_fastdiv(a.G);
+    a.by_nsplit = make_fastdiv(p.nsplit);
+    a.by_hd = make_fastdiv(a.c.hd);
     a.vec = aligned16(q_hi) && aligned16(q_lo) && ld % 4 == 0;
     a.first_wait_ns = first_wait_limit_ns();
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (p.nch == 1)
-        return p.rt == 1 ? ac_launch<1, 1, kAcW1, kAcS1>(a, p, s) : ac_launch<1, 2, kAcW1, kAcS1>(a, p, s);
-    return p.rt == 1 ? ac_launch<2, 1, kAcW2, kAcS2>(a, p, s) : ac_launch<2, 2, kAcW2, kAcS2>(a, p, s);
+    auto launch = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        return p.rt == 1 ? ac_launch<HD, 1>(a, p, s) : ac_launch<HD, 2>(a, p, s);
+    };
+    switch (a.c.hd) {
+    case 16: return launch(std::integral_constant<int, 16>());
+    case 32: return launch(std::integral_constant<int, 32>());
+    case 48: return launch(std::integral_constant<int, 48>());
+    case 64: return launch(std::integral_constant<int, 64>());
+    case 80: return launch(std::integral_constant<int, 80>());
+    case 96: return launch(std::integral_constant<int, 96>());
+    case 112: return launch(std::integral_constant<int, 112>());
+    default: return launch(std::integral_constant<int, 128>());
+    }
 }

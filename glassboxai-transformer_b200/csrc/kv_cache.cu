@@ -15,13 +15,31 @@ namespace gbx {
 
 constexpr float kTinyAmax = 7.888609052210118e-31f;   // 2^-100
 
-// The integer nearest to x / s, ties to even; rs = 1/s rounded.  s > 0.
-__device__ __forceinline__ int kv_code(float x, float s, float rs)
+// Four values' codes at scale s > 0 (rs = 1/s rounded), one to a byte: the
+// integers nearest to x / s, ties to even.  Adding 1.5 2^23 rounds x rs and
+// leaves the integer in the low mantissa bits.  Where a remainder reaches s/2
+// (a tie, or a neighbour of one: about one value in 10^5) the integer is
+// settled by it.
+constexpr float kKvMagic = 12582912.0f;
+
+__device__ __forceinline__ uint32_t kv_codes4(float4 x, float s, float rs)
 {
-    float q = rintf(x * rs);
-    const float r = fmaf(-q, s, x), h = 0.5f * s;
-    if (fabsf(r) > h || (fabsf(r) == h && ((int)q & 1))) q += copysignf(1.0f, r);
-    return (int)q;
+    const float2 magic = splat2(kKvMagic), by = splat2(rs), neg = splat2(-s);
+    float2 a = __ffma2_rn(lo2(x), by, magic), b = __ffma2_rn(hi2(x), by, magic);
+    const float2 qa = __fadd2_rn(a, splat2(-kKvMagic)), qb = __fadd2_rn(b, splat2(-kKvMagic));
+    const float2 ra = __ffma2_rn(qa, neg, lo2(x)), rb = __ffma2_rn(qb, neg, hi2(x));
+    const float h = 0.5f * s;
+    if (fmaxf(fmaxf(fabsf(ra.x), fabsf(ra.y)), fmaxf(fabsf(rb.x), fabsf(rb.y))) >= h) {
+        auto settle = [&](float& m, float q, float r) {
+            if (fabsf(r) > h || (fabsf(r) == h && ((int)q & 1))) m += copysignf(1.0f, r);
+        };
+        settle(a.x, qa.x, ra.x);
+        settle(a.y, qa.y, ra.y);
+        settle(b.x, qb.x, rb.x);
+        settle(b.y, qb.y, rb.y);
+    }
+    return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                       __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
 }
 
 // The page's scale for new values of largest size a; bad: one of them is not finite.
@@ -67,142 +85,313 @@ __device__ __forceinline__ KvBlock kv_block(const KvLayer& c, KvSeq q, int j)
 }
 
 // ---------------------------------------------------------------- append
-// One warp per (sequence, block, K or V, head): the largest |x| of the
-// block's new rows, the scale, the codes.  The rows are read twice, the
-// second time from L1.
-template <bool VEC>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvLayer c, const KvRows r, int64_t units, int blocks)
+struct KvAppend {
+    KvLayer c;
+    KvRows r;
+    FastDiv by_heads, by_blocks;   // unit = ((b * blocks + j) * 2 + which) * heads + h
+    int blocks;
+    uint32_t units;
+};
+
+struct KvUnit {
+    int h, which, j, b;
+};
+
+__device__ __forceinline__ KvUnit kv_unit(uint32_t u, int heads, FastDiv by_heads, int blocks, FastDiv by_blocks)
 {
-    grid_dependency_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (u >= units) return;
-    const int h = (int)(u % c.heads);
-    int64_t w = u / c.heads;
-    const int which = (int)(w & 1);
-    w >>= 1;
-    const int j = (int)(w % blocks), b = (int)(w / blocks);
-    bool bad_len;
-    const KvSeq q = kv_seq(c, b, &bad_len);
-    if (bad_len && lane == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
-    const KvBlock k = kv_block(c, q, j);
-    if (k.n <= 0) return;
-    const int page = kv_page(c, b, k.page_idx);
-    if (page < 0) {
-        if (lane == 0) kv_flag(c.err, GBX_KV_BAD_PAGE);
-        return;
+    KvUnit k;
+    const uint32_t w = fast_div(u, by_heads), v = w >> 1;
+    k.h = (int)(u - w * heads);
+    k.which = (int)(w & 1);
+    k.b = (int)fast_div(v, by_blocks);
+    k.j = (int)(v - k.b * blocks);
+    return k;
+}
+
+__device__ __forceinline__ float kv_abs4(float4 x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); }
+
+// 0, or NaN where an entry is not finite
+__device__ __forceinline__ float kv_bad4(float4 x) { return fmaf(x.x, 0.0f, fmaf(x.y, 0.0f, fmaf(x.z, 0.0f, x.w * 0.0f))); }
+
+template <bool VEC>
+__device__ __forceinline__ float4 kv_load4(const float* hi, const float* lo, int64_t at)
+{
+    float4 x;
+    if (VEC) {
+        x = *reinterpret_cast<const float4*>(hi + at);
+        if (lo) x = add4(x, *reinterpret_cast<const float4*>(lo + at));
+    } else {
+        x = make_float4(hi[at], hi[at + 1], hi[at + 2], hi[at + 3]);
+        if (lo) x = add4(x, make_float4(lo[at], lo[at + 1], lo[at + 2], lo[at + 3]));
     }
-    const int hd = c.hd, P = 1 << c.log_page;
-    const float* hi = r.hi[which] + ((int64_t)b * c.S + k.i0) * r.ld + (int64_t)h * hd;
-    const float* lo = r.lo[which] ? r.lo[which] + (hi - r.hi[which]) : nullptr;
-    const int64_t ph = (int64_t)page * c.heads + h;
-    int8_t* codes = (which ? c.v : c.k) + ph * P * hd;
-    float* scale = (which ? c.vs : c.ks) + ph;
-    const int quads = hd >> 2, n4 = k.n * quads;   // groups of 4 values
-    auto load = [&](int e) -> float4 {
-        const int64_t at = (int64_t)(e / quads) * r.ld + (e % quads) * 4;
-        float4 x;
-        if (VEC) {
-            x = *reinterpret_cast<const float4*>(hi + at);
-            if (lo) x = add4(x, *reinterpret_cast<const float4*>(lo + at));
-        } else {
-            x = make_float4(hi[at], hi[at + 1], hi[at + 2], hi[at + 3]);
-            if (lo) x = add4(x, make_float4(lo[at], lo[at + 1], lo[at + 2], lo[at + 3]));
-        }
-        return x;
-    };
-    float a = 0.0f;
-    bool bad = false;
-    for (int e = lane; e < n4; e += 32) {
-        const float4 x = load(e);
-        const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-        bad |= !(x.x - x.x == 0.0f) | !(x.y - x.y == 0.0f) | !(x.z - x.z == 0.0f) | !(x.w - x.w == 0.0f);
-        a = fmaxf(a, m);
-    }
-    a = group_max<32>(a);
-    bad = __any_sync(0xffffffffu, bad);
-    float s = kv_new_scale(a, bad);
+    return x;
+}
+
+// The page's scale with new values of largest size amax in, and where it grew
+// the codes of the slots before slot s0 recoded by `threads` threads, this one
+// the id-th.  Called by all of them, which have to meet before *scale is stored.
+__device__ __forceinline__ float kv_grow(const KvBlock& k, int8_t* codes, const float* scale, float amax, bool bad, int which, int hd,
+                                         int id, int threads)
+{
+    float s = kv_new_scale(amax, bad);
     if (k.s0 > 0) {
         const float old = *scale;
         s = kv_max_scale(old, s);
-        if (s != old) {   // grew, or turned NaN: the earlier slots' codes
-            for (int e = lane; e < k.s0 * hd; e += 32) {
+        if (s != old) {   // grew, or turned NaN
+            for (int e = id; e < k.s0 * hd; e += threads) {
                 const int t = e / hd, i = e % hd;
                 int8_t* p = codes + (which ? ((t >> 4) * hd + i) * 16 + (t & 15) : t * hd + i);
                 *p = (int8_t)(s > 0.0f ? kv_recode(*p, old, s) : 0);
             }
         }
     }
+    return s;
+}
+
+// Few new rows per sequence (a decode step, drafts): one warp per (sequence, block, K or V, head), the
+// largest |x| of the block's new rows, the scale, the codes.  The rows are
+// read twice, the second time from L1.  Latency bounds it (length, page, rows,
+// codes one after another): 3.5 us for 32 sequences x 12 heads, 10 for 256 x 25.
+template <bool VEC>
+__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppend a)
+{
+    grid_dependency_wait();
+    const KvLayer& c = a.c;
+    const int lane = threadIdx.x & 31;
+    const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= a.units) return;
+    const KvUnit u = kv_unit(unit, c.heads, a.by_heads, a.blocks, a.by_blocks);
+    bool bad_len;
+    const KvSeq q = kv_seq(c, u.b, &bad_len);
+    if (bad_len && lane == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
+    const KvBlock k = kv_block(c, q, u.j);
+    if (k.n <= 0) return;
+    const int page = kv_page(c, u.b, k.page_idx);
+    if (page < 0) {
+        if (lane == 0) kv_flag(c.err, GBX_KV_BAD_PAGE);
+        return;
+    }
+    const int hd = c.hd;
+    const float* base = a.r.hi[u.which];
+    const float* hi = base + ((int64_t)u.b * c.S + k.i0) * a.r.ld + (int64_t)u.h * hd;
+    const float* lo = a.r.lo[u.which] ? a.r.lo[u.which] + (hi - base) : nullptr;
+    const int64_t ph = (int64_t)page * c.heads + u.h;
+    int8_t* codes = (u.which ? c.v : c.k) + (ph << c.log_page) * hd;
+    float* scale = (u.which ? c.vs : c.ks) + ph;
+    const int quads = hd >> 2, n4 = k.n * quads;   // groups of 4 values
+    float amax = 0.0f, bad = 0.0f;
+    for (int e = lane; e < n4; e += 32) {
+        const float4 x = kv_load4<VEC>(hi, lo, (int64_t)(e / quads) * a.r.ld + (e % quads) * 4);
+        amax = fmaxf(amax, kv_abs4(x));
+        bad += kv_bad4(x);
+    }
+    amax = group_max<32>(amax);
+    const float s = kv_grow(k, codes, scale, amax, __any_sync(0xffffffffu, bad != bad), u.which, hd, lane, 32);
     __syncwarp();
     if (lane == 0) *scale = s;
     const bool live = s > 0.0f;   // false for 0 and NaN: codes 0
     const float rs = 1.0f / s;
     for (int e = lane; e < n4; e += 32) {
-        const float4 x = load(e);
-        const int t = k.s0 + e / quads, i = (e % quads) * 4;
-        char4 q4 = make_char4(0, 0, 0, 0);
-        if (live) {
-            q4.x = (signed char)kv_code(x.x, s, rs);
-            q4.y = (signed char)kv_code(x.y, s, rs);
-            q4.z = (signed char)kv_code(x.z, s, rs);
-            q4.w = (signed char)kv_code(x.w, s, rs);
-        }
-        if (which) {
+        const int r = e / quads, i = (e - r * quads) * 4, t = k.s0 + r;
+        const float4 x = kv_load4<VEC>(hi, lo, (int64_t)r * a.r.ld + i);
+        const uint32_t q4 = live ? kv_codes4(x, s, rs) : 0u;
+        if (u.which) {
             int8_t* p = codes + ((t >> 4) * hd + i) * 16 + (t & 15);
-            p[0] = q4.x;
-            p[16] = q4.y;
-            p[32] = q4.z;
-            p[48] = q4.w;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) p[16 * m] = (int8_t)(q4 >> (8 * m));
         } else {
-            *reinterpret_cast<char4*>(codes + t * hd + i) = q4;
+            *reinterpret_cast<uint32_t*>(codes + t * hd + i) = q4;
+        }
+    }
+}
+
+// Many new rows: one CTA per (sequence, block, K or V, head), a warp for every
+// 16 slots x 64 columns, 32 values to a lane held in registers between the
+// maximum and the codes, so each row is read once.  Keys: a lane has four
+// columns of every other slot (16-byte loads, 4-byte stores, a row's in
+// line); values: two columns of all 16 slots, whose codes are two 16-byte words
+// of the 16-tokens-innermost layout.  HBM bounds it: 32.5 us for 8 prompts of 1024
+// rows of 25 heads x 64 (131 MB, 4.0 TB/s), the rest the CTAs' start.
+template <bool VEC>
+__global__ void __launch_bounds__(512) kv_append_pages_kernel(const KvAppend a)
+{
+    grid_dependency_wait();
+    __shared__ float s_max[16], s_bad[16];
+    const KvLayer& c = a.c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const KvUnit u = kv_unit(blockIdx.x, c.heads, a.by_heads, a.blocks, a.by_blocks);
+    bool bad_len;
+    const KvSeq q = kv_seq(c, u.b, &bad_len);
+    if (bad_len && threadIdx.x == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
+    const KvBlock k = kv_block(c, q, u.j);
+    if (k.n <= 0) return;
+    const int hd = c.hd;
+    const int page = kv_page(c, u.b, k.page_idx);   // not waited for before the rows are asked for
+    // this warp's slots t0 .. t0 + 15 and columns c0 .. c0 + 63
+    const int halves = hd > 64 ? 2 : 1;
+    const int t0 = 16 * (halves == 2 ? warp >> 1 : warp), c0 = halves == 2 ? 64 * (warp & 1) : 0;
+    const float* base = a.r.hi[u.which];
+    // row of slot 0 (which may lie before the call's rows)
+    const float* hi = base + ((int64_t)u.b * c.S + k.i0 - k.s0) * a.r.ld + (int64_t)u.h * hd;
+    const float* lo = a.r.lo[u.which] ? a.r.lo[u.which] + (hi - base) : nullptr;
+    const int ks0 = k.s0, ks1 = k.s0 + k.n;   // the slots to be filled
+    // values: x[i] = slots 2i, 2i + 1 x two columns.  All of a plane's loads are
+    // issued before any is used.
+    const int col = u.which ? c0 + 2 * lane : c0 + 4 * (lane & 15);
+    const bool in = col < hd;
+    auto plane = [&](const float* src, float4 (&x)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (u.which == 0) {
+                const int t = t0 + 2 * i + (lane >> 4);
+                const float* at = src + t * a.r.ld + col;
+                if (in && t >= ks0 && t < ks1) x[i] = VEC ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+            } else {
+                const int t = t0 + 2 * i;
+                const float* at = src + t * a.r.ld + col;
+                float2 y = make_float2(0.0f, 0.0f), z = y;
+                if (in && t >= ks0 && t < ks1) y = VEC ? *reinterpret_cast<const float2*>(at) : make_float2(at[0], at[1]);
+                at += a.r.ld;
+                if (in && t + 1 >= ks0 && t + 1 < ks1) z = VEC ? *reinterpret_cast<const float2*>(at) : make_float2(at[0], at[1]);
+                x[i] = cat2(y, z);
+            }
+        }
+    };
+    float4 x[8];
+    plane(hi, x);
+    if (lo) {
+        float4 y[8];
+        plane(lo, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = add4(x[i], y[i]);
+    }
+    float amax = 0.0f, bad = 0.0f;
+    if (page < 0) {   // the CTA's threads alike
+        if (threadIdx.x == 0) kv_flag(c.err, GBX_KV_BAD_PAGE);
+        return;
+    }
+    const int64_t ph = (int64_t)page * c.heads + u.h;
+    int8_t* codes = (u.which ? c.v : c.k) + (ph << c.log_page) * hd;
+    float* scale = (u.which ? c.vs : c.ks) + ph;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        amax = fmaxf(amax, kv_abs4(x[i]));
+        bad += kv_bad4(x[i]);
+    }
+    amax = group_max<32>(amax);
+    bad = group_sum<32>(bad);
+    if (lane == 0) {
+        s_max[warp] = amax;
+        s_bad[warp] = bad;
+    }
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) {
+        amax = fmaxf(amax, s_max[w]);
+        bad += s_bad[w];
+    }
+    const float s = kv_grow(k, codes, scale, amax, bad != bad, u.which, hd, threadIdx.x, blockDim.x);
+    __syncthreads();   // every thread has read the old scale, and recoded what it recodes
+    if (threadIdx.x == 0) *scale = s;
+    if (col >= hd) return;
+    const bool live = s > 0.0f;
+    const float rs = 1.0f / s;
+    uint32_t q4[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        q4[i] = live ? kv_codes4(x[i], s, rs) : 0u;
+    if (u.which == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = t0 + 2 * i + (lane >> 4);
+            if (t >= ks0 && t < ks1) *reinterpret_cast<uint32_t*>(codes + t * hd + col) = q4[i];
+        }
+    } else {
+        // q4[i]: bytes (slot 2i: columns 0, 1; slot 2i + 1: columns 0, 1)
+        int8_t* to = codes + ((t0 >> 4) * hd + col) * 16;
+        uint32_t w[2][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[0][i] = __byte_perm(q4[2 * i], q4[2 * i + 1], 0x6420);
+            w[1][i] = __byte_perm(q4[2 * i], q4[2 * i + 1], 0x7531);
+        }
+        if (ks0 <= t0 && t0 + 16 <= ks1) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+            *reinterpret_cast<uint4*>(to + 16) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                if (t0 + t >= ks0 && t0 + t < ks1) {
+                    to[t] = (int8_t)(w[0][t >> 2] >> (8 * (t & 3)));
+                    to[16 + t] = (int8_t)(w[1][t >> 2] >> (8 * (t & 3)));
+                }
         }
     }
 }
 
 // ---------------------------------------------------------------- read back
-// One thread per four values of a row.
+// One warp per (sequence, 16-token group, K or V, head).  Keys: a lane takes four
+// columns of a token; values: one column of all 16 tokens, a 16-byte load, and
+// stores row by row, 32 columns in line.  HBM bounds it: 5.1 TB/s for 8 x 1087 rows
+// of 25 heads x 64; five CTAs to an SM (8 with spills 4.1, 3 by registers 2.7).
 template <bool VEC>
-__global__ void __launch_bounds__(256)
-kv_read_kernel(const KvLayer c, float* k_out, float* v_out, int64_t ld, int64_t units)
+__global__ void __launch_bounds__(256, 5)
+kv_read_kernel(const KvLayer c, float* k_out, float* v_out, int64_t ld, FastDiv by_heads, int groups, FastDiv by_groups, FastDiv by_quads, uint32_t units)
 {
     grid_dependency_wait();
-    const int quads = c.hd >> 2, row4 = c.heads * quads;
-    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
-        const int64_t row = u / row4;
-        const int x = (int)(u - row * row4), h = x / quads, i = (x - h * quads) * 4;
-        const int b = (int)(row / c.S), ri = (int)(row - (int64_t)b * c.S);
-        bool bad_len;
-        const KvSeq q = kv_seq(c, b, &bad_len);
-        if (bad_len && ri == 0 && x == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
-        if (ri >= q.n) continue;
-        const int t = q.len - q.n + ri, P = 1 << c.log_page, slot = t & (P - 1);
-        const int page = kv_page(c, b, t >> c.log_page);
-        if (page < 0) {
-            if (x == 0) kv_flag(c.err, GBX_KV_BAD_PAGE);
-            continue;
+    const int lane = threadIdx.x & 31;
+    const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= units) return;
+    const KvUnit u = kv_unit(unit, c.heads, by_heads, groups, by_groups);
+    bool bad_len;
+    const KvSeq q = kv_seq(c, u.b, &bad_len);
+    if (bad_len && lane == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
+    const int first = q.len - q.n;                  // the first token wanted
+    const int g = (first >> 4) + u.j, t0 = 16 * g;  // this group's first token
+    float* out = u.which ? v_out : k_out;
+    if (q.n == 0 || t0 >= q.len || !out) return;
+    const int page = kv_page(c, u.b, t0 >> c.log_page);
+    if (page < 0) {
+        if (lane == 0) kv_flag(c.err, GBX_KV_BAD_PAGE);
+        return;
+    }
+    const int hd = c.hd;
+    const int64_t ph = (int64_t)page * c.heads + u.h;
+    const float s = (u.which ? c.vs : c.ks)[ph];
+    const int8_t* p = (u.which ? c.v : c.k) + (ph << c.log_page) * hd + (t0 & ((1 << c.log_page) - 1)) * hd;
+    float* o = out + ((int64_t)u.b * c.S + t0 - first) * ld + (int64_t)u.h * hd;   // row of token t0
+    const int lo = max(0, first - t0), hi = min(16, q.len - t0);                  // the group's tokens wanted
+    if (u.which) {
+        for (int col = lane; col < hd; col += 32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p + col * 16);
+            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+            float* to = o + col;
+#pragma unroll
+            for (int t = 0; t < 16; ++t, to += ld)
+                if (t >= lo && t < hi) *to = (float)(int8_t)(x[t >> 2] >> (8 * (t & 3))) * s;
         }
-        const int64_t ph = (int64_t)page * c.heads + h;
-        for (int which = 0; which < 2; ++which) {
-            float* out = which ? v_out : k_out;
-            if (!out) continue;
-            const float s = (which ? c.vs : c.ks)[ph];
-            const int8_t* p = (which ? c.v : c.k) + ph * P * c.hd;
-            char4 q4;
-            if (which) {
-                p += ((slot >> 4) * c.hd + i) * 16 + (slot & 15);
-                q4 = make_char4(p[0], p[16], p[32], p[48]);
-            } else {
-                q4 = *reinterpret_cast<const char4*>(p + slot * c.hd + i);
-            }
-            const float4 f = make_float4(q4.x * s, q4.y * s, q4.z * s, q4.w * s);
-            float* o = out + row * ld + (int64_t)h * c.hd + i;
-            if (VEC) {
-                *reinterpret_cast<float4*>(o) = f;
-            } else {
-                o[0] = f.x;
-                o[1] = f.y;
-                o[2] = f.z;
-                o[3] = f.w;
+    } else {
+        // 128 values at a time: 8 x 16 columns are 4 loads of a lane ahead of their stores
+        const int quads = hd >> 2, all = 16 * quads;
+        for (int e0 = lane; e0 < all; e0 += 128) {
+            char4 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e0 + 32 * i < all) w[i] = *reinterpret_cast<const char4*>(p + 4 * (e0 + 32 * i));   // codes of a group are contiguous
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = e0 + 32 * i, t = (int)fast_div(e, by_quads), c4 = (e - t * quads) * 4;
+                if (e >= all || t < lo || t >= hi) continue;
+                float* to = o + t * ld + c4;
+                const float4 f = make_float4(w[i].x * s, w[i].y * s, w[i].z * s, w[i].w * s);
+                if (VEC) {
+                    *reinterpret_cast<float4*>(to) = f;
+                } else {
+                    to[0] = f.x;
+                    to[1] = f.y;
+                    to[2] = f.z;
+                    to[3] = f.w;
+                }
             }
         }
     }
@@ -220,7 +409,7 @@ struct KvPool {
     int32_t* err;
 };
 
-// One CTA per (pair, layer, K or V).  A page of a layer is one contiguous
+// One CTA per (pair, layer, K or V): 6.0 TB/s at 600 pages of 24 layers.  A page of a layer is one contiguous
 // run of bytes.  Before it stores, the CTA looks its target up among all
 // sources and earlier targets (n words each, from L2): a pair that would race
 // with another is left out, by every CTA alike.
@@ -312,7 +501,7 @@ extern "C" int gbx_kv_append(const gbx_kv_cache* cache_host, int layer, const in
                              const float* k_lo, const float* v_hi, const float* v_lo, int64_t ld, int* err_flag,
                              gbx_stream_t stream)
 {
-    KvLayer c;
+    KvLayer c = {};
     if (int rc = kv_layer(cache_host, layer, table, max_pages, kv_len, n_new, B, S, err_flag, "gbx_kv_append", &c))
         return rc;
     if (B == 0 || S == 0) return GBX_OK;
@@ -324,18 +513,32 @@ extern "C" int gbx_kv_append(const gbx_kv_cache* cache_host, int layer, const in
     const int64_t touched = ((int64_t)S + 2 * P - 2) / P;
     const int blocks = (int)(touched < max_pages ? touched : max_pages);
     const int64_t units = (int64_t)B * blocks * 2 * c.heads;
-    if ((units + 7) / 8 > 0x7fffffffLL) return set_error(GBX_ERANGE, "gbx_kv_append: B=%d S=%d heads=%d", B, S, c.heads);
-    KvRows r;
-    r.hi[0] = k_hi;
-    r.hi[1] = v_hi;
-    r.lo[0] = k_lo;
-    r.lo[1] = v_lo;
-    r.ld = ld;
+    if (units > 0x7fffffffLL - 8) return set_error(GBX_ERANGE, "gbx_kv_append: B=%d S=%d heads=%d", B, S, c.heads);
+    KvAppend a;
+    a.c = c;
+    a.r.hi[0] = k_hi;
+    a.r.hi[1] = v_hi;
+    a.r.lo[0] = k_lo;
+    a.r.lo[1] = v_lo;
+    a.r.ld = ld;
+    a.by_heads = make_fastdiv(c.heads);
+    a.by_blocks = make_fastdiv(blocks);
+    a.blocks = blocks;
+    a.units = (uint32_t)units;
     const bool vec = aligned16(k_hi) && aligned16(v_hi) && aligned16(k_lo) && aligned16(v_lo) && ld % 4 == 0;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)((units + 7) / 8));
-    if (vec) launch_row_kernel(kv_append_kernel<true>, grid, dim3(256), 0, s, c, r, units, blocks);
-    else launch_row_kernel(kv_append_kernel<false>, grid, dim3(256), 0, s, c, r, units, blocks);
+    // Whole pages pay for a CTA each: 256 rows of 25 heads x 64 at 16 rows a sequence and
+    // 64 to a page take 13 us by rows and 27 by pages, at 32 rows 27 and 28; 64 rows at 16 to a
+    // page 34 and 22, 8 prompts of 1024 rows at 64 101 and 33.
+    if (S < 32 || S < P) {
+        const dim3 grid((unsigned)((units + 7) / 8));
+        if (vec) launch_row_kernel(kv_append_kernel<true>, grid, dim3(256), 0, s, a);
+        else launch_row_kernel(kv_append_kernel<false>, grid, dim3(256), 0, s, a);
+    } else {
+        const dim3 block((unsigned)(32 * (P / 16) * (c.hd > 64 ? 2 : 1)));
+        if (vec) launch_row_kernel(kv_append_pages_kernel<true>, dim3((unsigned)units), block, 0, s, a);
+        else launch_row_kernel(kv_append_pages_kernel<false>, dim3((unsigned)units), block, 0, s, a);
+    }
     return check_launch("gbx_kv_append");
 }
 
@@ -343,18 +546,25 @@ extern "C" int gbx_kv_read(const gbx_kv_cache* cache_host, int layer, const int3
                            const int32_t* kv_len, const int32_t* n, int B, int S, float* k_out, float* v_out,
                            int64_t ld, int* err_flag, gbx_stream_t stream)
 {
-    KvLayer c;
+    KvLayer c = {};
     if (int rc = kv_layer(cache_host, layer, table, max_pages, kv_len, n, B, S, err_flag, "gbx_kv_read", &c)) return rc;
     if (B == 0 || S == 0 || (!k_out && !v_out)) return GBX_OK;
     if (ld < (int64_t)c.heads * c.hd) return set_error(GBX_EINVAL, "gbx_kv_read: ld=%lld < heads*hd", (long long)ld);
-    const int64_t units = (int64_t)B * S * c.heads * (c.hd / 4);
-    const bool vec = aligned16(k_out) && aligned16(v_out) && ld % 4 == 0;
+    // 16-token groups that S tokens can touch
+    const int64_t touched = ((int64_t)S + 30) / 16, most = (int64_t)max_pages << (c.log_page - 4);
+    const int groups = (int)(touched < most ? touched : most);
+    const int64_t units = (int64_t)B * groups * 2 * c.heads;
+    if (units > 0x7fffffffLL - 8) return set_error(GBX_ERANGE, "gbx_kv_read: B=%d S=%d heads=%d", B, S, c.heads);
+    const bool vec = aligned16(k_out) && ld % 4 == 0;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const int grid = vec ? persistent_grid(kv_read_kernel<true>, 256, 0, (units + 255) / 256, 8)
-                         : persistent_grid(kv_read_kernel<false>, 256, 0, (units + 255) / 256, 8);
-    if (grid < 0) return GBX_ECUDA;
-    if (vec) launch_row_kernel(kv_read_kernel<true>, dim3(grid), dim3(256), 0, s, c, k_out, v_out, ld, units);
-    else launch_row_kernel(kv_read_kernel<false>, dim3(grid), dim3(256), 0, s, c, k_out, v_out, ld, units);
+    const dim3 grid((unsigned)((units + 7) / 8));
+    const FastDiv by_heads = make_fastdiv(c.heads), by_groups = make_fastdiv(groups), by_quads = make_fastdiv(c.hd / 4);
+    if (vec)
+        launch_row_kernel(kv_read_kernel<true>, grid, dim3(256), 0, s, c, k_out, v_out, ld, by_heads, groups, by_groups,
+                          by_quads, (uint32_t)units);
+    else
+        launch_row_kernel(kv_read_kernel<false>, grid, dim3(256), 0, s, c, k_out, v_out, ld, by_heads, groups, by_groups,
+                          by_quads, (uint32_t)units);
     return check_launch("gbx_kv_read");
 }
 

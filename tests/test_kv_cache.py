@@ -13,7 +13,7 @@ class _Cache:
         import ctypes
         v = dict(k=1 << 20, v=2 << 20, k_scale=3 << 20, v_scale=4 << 20, pages=8, layers=2, page=16, heads=2, hd=64)
         v.update(kw)
-        self.device, self.heads = None, v["heads"]
+        self.device, self._dev, self.heads = None, -1, v["heads"]
         self._c = gbx._KVCacheStruct(v["k"], v["v"], v["k_scale"], v["v_scale"], v["pages"], v["layers"], v["page"], v["heads"], v["hd"])
         self._ref = ctypes.byref(self._c)
 
@@ -85,7 +85,7 @@ def test_bad_calls_are_refused(gbx):
     _refused(gbx, lambda: gbx.verify_tokens(16, 16, 16, 16, temperature=float("inf"), **ver), 1, "temperature")
     _refused(gbx, lambda: gbx.verify_tokens(16, 16, 16, 16, **dict(ver, vocab=0)), 1, "vocab")
     _refused(gbx, lambda: gbx.verify_tokens(16, 16, 16, 16, **dict(ver, n_draft=-1)), 1, "n_draft")
-    _refused(gbx, lambda: gbx.verify_tokens(16, 16, 16, 16, **dict(ver, n_draft=1025)), 3, "n_draft")
+    _refused(gbx, lambda: gbx.verify_tokens(16, 16, 16, 16, **dict(ver, n_draft=257)), 3, "n_draft")
 
 
 def test_empty_calls_do_nothing(gbx):
