@@ -18,7 +18,7 @@
 // second one holds digit 2 (for 16 query rows: their digits 2 side by side),
 // so the thread that holds a row's digit-0 sum holds the others.  The integer
 // accumulators start at the bits of 1.5 2^23: the sums, below 2^22 in size,
-// are then read as floats with one subtraction.
+// are then read as floats.
 //
 // One warp takes 64 tokens a step, four 16-token groups that each lie in one
 // page.  Lane (n, c) = (lane / 4, lane % 4) reads 16 key bytes of one token,
@@ -75,7 +75,7 @@ struct AcArgs {
     int nrb;          // row blocks per (sequence, key head)
     int nsplit;       // clusters per unit
     FastDiv by_heads, by_nrb, by_g, by_nsplit, by_hd;
-    int vec;          // q rows are 16-byte aligned
+    int vec, vec_out; // the rows of q, of out and out_lo are 16-byte aligned
     uint64_t first_wait_ns;
 };
 
@@ -123,7 +123,7 @@ __device__ __forceinline__ uint4 ac_lds(uint32_t at)
 // before every use.
 struct AcConst {
     uint32_t c[4], z[2];
-    float2 less, by, two23;
+    float2 less, less257, less65793, by, by2, two23;
     __device__ __forceinline__ static float reg(float x)
     {
         float y;
@@ -138,18 +138,27 @@ struct AcConst {
         for (int i = 0; i < 2; ++i) asm volatile("mov.u32 %0, 0;" : "=r"(z[i]));
         less = make_float2(reg(-kAcMagicF), reg(-kAcMagicF));
         by = make_float2(reg(256.0f), reg(256.0f));
+        less257 = make_float2(reg(-257.0f * kAcMagicF), reg(-257.0f * kAcMagicF));
+        less65793 = make_float2(reg(-65793.0f * kAcMagicF), reg(-65793.0f * kAcMagicF));
+        by2 = make_float2(reg(65536.0f), reg(65536.0f));
         two23 = make_float2(reg(8388608.0f), reg(8388608.0f));
     }
 };
 
 // 65536 s2 + 256 s1 + s0 of accumulators that started at 0x4b400000, two
-// neighbouring columns at a time (packed fp32, two lanes an instruction).
+// neighbouring columns at a time (packed fp32, two lanes an instruction).  f_i =
+// M + s_i with M = 1.5 2^23.  For the weights (U) M leaves s2 before the sum, so
+// that only the sum's own roundings are left.  For the scores it leaves with one
+// constant, -65793 M; that rounds to a multiple of 256 where the query's own
+// rounding already cost about 500.
+template <bool U>
 __device__ __forceinline__ float2 ac_join(uint32_t s0, uint32_t t0, uint32_t s1, uint32_t t1, uint32_t s2, uint32_t t2, const AcConst& k)
 {
-    const float2 f0 = __fadd2_rn(make_float2(__uint_as_float(s0), __uint_as_float(t0)), k.less);
-    const float2 f1 = __fadd2_rn(make_float2(__uint_as_float(s1), __uint_as_float(t1)), k.less);
-    const float2 f2 = __fadd2_rn(make_float2(__uint_as_float(s2), __uint_as_float(t2)), k.less);
-    return __ffma2_rn(__ffma2_rn(f2, k.by, f1), k.by, f0);
+    const float2 f0 = make_float2(__uint_as_float(s0), __uint_as_float(t0));
+    const float2 f1 = make_float2(__uint_as_float(s1), __uint_as_float(t1));
+    const float2 f2 = make_float2(__uint_as_float(s2), __uint_as_float(t2));
+    if (U) return __fadd2_rn(__ffma2_rn(__fadd2_rn(f2, k.less), k.by2, __ffma2_rn(f1, k.by, k.less257)), f0);
+    return __fadd2_rn(__ffma2_rn(f1, k.by, __ffma2_rn(f2, k.by2, k.less65793)), f0);
 }
 
 // 32-column blocks of a head, in pairs: a lane's 16 key bytes feed two.
@@ -185,7 +194,7 @@ __device__ __forceinline__ void ac_dot(float2 (&s)[RT], const AcDigits<RT, M>& a
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        s[rt] = ac_join(x[rt][0], x[rt][1], x[rt][2], x[rt][3], y[2 * rt], y[2 * rt + 1], k);
+        s[rt] = ac_join<U>(x[rt][0], x[rt][1], x[rt][2], x[rt][3], y[2 * rt], y[2 * rt + 1], k);
     }
 }
 
@@ -203,7 +212,7 @@ __device__ __forceinline__ AcUnit ac_unit(const AcArgs& a, uint32_t unit, int R,
     u.h = (int)(unit - w * a.c.heads);
     u.b = (int)fast_div(w, a.by_nrb);
     u.seq = kv_seq(a.c, u.b, bad_len);
-    u.r0 = (int)(w - u.b * a.nrb) * R;
+    u.r0 = (a.nrb - 1 - (int)(w - u.b * a.nrb)) * R;   // the rows that see most first
     u.rows = min(R, u.seq.n * a.G - u.r0);   // valid rows of this block, if positive
     return u;
 }
@@ -224,6 +233,28 @@ __device__ __forceinline__ void ac_store(const AcArgs& a, int64_t at, float v)
         a.out_lo[at] = vl;
     } else {
         a.out[at] = v;
+    }
+}
+
+// Four neighbouring columns of an output row: acc / sum, 0 for a row that saw nothing.
+__device__ __forceinline__ void ac_store4(const AcArgs& a, int64_t at, float4 acc, float sum)
+{
+    const float4 v = sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                 : make_float4(acc.x / sum, acc.y / sum, acc.z / sum, acc.w / sum);
+    if (a.vec_out) {
+        if (a.out_lo) {
+            float4 vh, vl;
+            split4(v, vh, vl);
+            *reinterpret_cast<float4*>(a.out + at) = vh;
+            *reinterpret_cast<float4*>(a.out_lo + at) = vl;
+        } else {
+            *reinterpret_cast<float4*>(a.out + at) = v;
+        }
+    } else {
+        ac_store(a, at, v.x);
+        ac_store(a, at + 1, v.y);
+        ac_store(a, at + 2, v.z);
+        ac_store(a, at + 3, v.w);
     }
 }
 
@@ -388,6 +419,249 @@ __device__ __forceinline__ void ac_values(uint32_t vb, const AcDigits<RT, 2>& p,
     }
 }
 
+// Where the rows' partial results meet: NW partial results of R rows (one per
+// warp, or one that the warps fill together) and the CTA's own after them, in
+// the shared memory that held the ring.
+template <int HD, int R, int NW>
+struct AcMeet {
+    float *o, *m, *l;   // [NW + 1][R][HD], [NW + 1][R] twice
+    __device__ __forceinline__ explicit AcMeet(uint8_t* smem)
+        : o(reinterpret_cast<float*>(smem)), m(o + (NW + 1) * R * HD), l(m + (NW + 1) * R)
+    {
+    }
+
+    // this warp's rows base .. base + 8 RT - 1, into partial result w
+    template <int RT>
+    __device__ __forceinline__ void put(int w, int base, int rows, const float (&mm)[RT], float (&ll)[RT], const float2 (&oo)[RT][HD / 8])
+    {
+        const int lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            ll[rt] += __shfl_xor_sync(0xffffffffu, ll[rt], 1);
+            ll[rt] += __shfl_xor_sync(0xffffffffu, ll[rt], 2);
+            const int r = base + 8 * rt + n;
+            if (r < rows) {
+                if (cc == 0) {
+                    m[w * R + r] = mm[rt];
+                    l[w * R + r] = ll[rt];
+                }
+#pragma unroll
+                for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<float2*>(o + (w * R + r) * HD + 8 * j + 2 * cc) = oo[rt][j];
+            }
+        }
+    }
+
+    // The partial results' sum: to the output, or with more CTAs at work on the
+    // unit through the cluster's shared memory to the output or the workspace.  For
+    // the few rows of the splitting kernel, one column to a thread: there the form
+    // below costs the kernel's loop 40 registers (256 sequences x 25 heads x 2048
+    // tokens 279 us against 255), and gains nothing.
+    __device__ __forceinline__ void finish_few(const AcArgs& a, const AcUnit& u, uint32_t unit, int split, uint32_t rank, uint32_t csize, int threads)
+    {
+        const int nr = u.rows;
+        const bool alone = csize == 1 && a.nsplit == 1;
+        for (int e = threadIdx.x; e < nr * HD; e += threads) {
+            const int r = e / HD, col = e - r * HD;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) mx = fmaxf(mx, m[w * R + r]);
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            float acc = 0.0f, ll = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = ac_exp2(m[w * R + r] - base);
+                acc += f * o[(w * R + r) * HD + col];
+                ll += f * l[w * R + r];
+            }
+            if (alone) {
+                ac_store(a, ac_row(a, u, r, a.ld_out) + col, ll == 0.0f ? 0.0f : acc / ll);
+            } else {
+                o[(NW * R + r) * HD + col] = acc;
+                if (col == 0) {
+                    m[NW * R + r] = mx;
+                    l[NW * R + r] = ll;
+                }
+            }
+        }
+        if (alone) return;
+        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+        auto peer = [&](uint32_t p, const float* x) -> float {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc::mapa(tc::smem_u32(x), p)) : "memory");
+            return v;
+        };
+        for (int e = (int)rank * threads + threadIdx.x; e < nr * HD; e += (int)csize * threads) {
+            const int r = e / HD, col = e - r * HD;
+            float mx = -INFINITY;
+            for (uint32_t p = 0; p < csize; ++p) mx = fmaxf(mx, peer(p, m + NW * R + r));
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            float acc = 0.0f, ll = 0.0f;
+            for (uint32_t p = 0; p < csize; ++p) {
+                const float f = ac_exp2(peer(p, m + NW * R + r) - base);
+                acc += f * peer(p, o + (NW * R + r) * HD + col);
+                ll += f * peer(p, l + NW * R + r);
+            }
+            if (a.nsplit == 1) {
+                ac_store(a, ac_row(a, u, r, a.ld_out) + col, ll == 0.0f ? 0.0f : acc / ll);
+            } else {
+                float* w = a.ws + ((int64_t)unit * a.nsplit + split) * (R * (HD + 2));
+                w[r * HD + col] = acc;
+                if (col == 0) {
+                    w[R * HD + r] = mx;
+                    w[R * HD + R + r] = ll;
+                }
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    }
+
+    // The same for many rows (300 rows of 12 heads over 4000 tokens: 35 us
+    // against 40).  The factors that bring the partial results to one maximum are formed once
+    // a row; then every thread takes four columns of a row at a time.
+    __device__ __forceinline__ void finish(const AcArgs& a, const AcUnit& u, uint32_t unit, int split, uint32_t rank, uint32_t csize, int threads)
+    {
+        constexpr int Q = HD / 4;
+        const int nr = u.rows;
+        const bool alone = csize == 1 && a.nsplit == 1;
+        for (int r = threadIdx.x; r < nr; r += threads) {
+            float mx = m[r];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) mx = fmaxf(mx, m[w * R + r]);
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            float ll = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = ac_exp2(m[w * R + r] - base);
+                ll += f * l[w * R + r];
+                m[w * R + r] = f;
+            }
+            m[NW * R + r] = mx;
+            l[NW * R + r] = ll;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < nr * Q; e += threads) {
+            const int r = e / Q, col = 4 * (e - r * Q);
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < NW; ++w) acc = fma4s(*reinterpret_cast<const float4*>(o + (w * R + r) * HD + col), m[w * R + r], acc);
+            if (alone) ac_store4(a, ac_row(a, u, r, a.ld_out) + col, acc, l[NW * R + r]);
+            else *reinterpret_cast<float4*>(o + (NW * R + r) * HD + col) = acc;
+        }
+        if (alone) return;
+        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+        auto at = [&](uint32_t p, const float* x) { return tc::mapa(tc::smem_u32(x), p); };
+        auto peer = [&](uint32_t p, const float* x) -> float {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at(p, x)) : "memory");
+            return v;
+        };
+        // factors [csize][R] in place of the first partial results, and the sums
+        float* f = o;
+        for (int r = threadIdx.x; r < nr; r += threads) {
+            float pm[kAcMaxCluster], pl[kAcMaxCluster];
+            float mx = -INFINITY;
+#pragma unroll
+            for (uint32_t p = 0; p < kAcMaxCluster; ++p)
+                if (p < csize) {
+                    pm[p] = peer(p, m + NW * R + r);
+                    pl[p] = peer(p, l + NW * R + r);
+                }
+#pragma unroll
+            for (uint32_t p = 0; p < kAcMaxCluster; ++p)
+                if (p < csize) mx = fmaxf(mx, pm[p]);
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            float ll = 0.0f;
+#pragma unroll
+            for (uint32_t p = 0; p < kAcMaxCluster; ++p)
+                if (p < csize) {
+                    const float x = ac_exp2(pm[p] - base);
+                    f[p * R + r] = x;
+                    ll += x * pl[p];
+                }
+            m[r] = mx;
+            l[r] = ll;
+        }
+        __syncthreads();
+        float* w = a.ws + ((int64_t)unit * a.nsplit + split) * (R * (HD + 2));
+        for (int e = (int)rank * threads + threadIdx.x; e < nr * Q; e += (int)csize * threads) {
+            const int r = e / Q, col = 4 * (e - r * Q);
+            float4 v[kAcMaxCluster];
+#pragma unroll
+            for (uint32_t p = 0; p < kAcMaxCluster; ++p)
+                if (p < csize)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                                 : "=f"(v[p].x), "=f"(v[p].y), "=f"(v[p].z), "=f"(v[p].w)
+                                 : "r"(at(p, o + (NW * R + r) * HD + col))
+                                 : "memory");
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t p = 0; p < kAcMaxCluster; ++p)
+                if (p < csize) acc = fma4s(v[p], f[p * R + r], acc);
+            if (a.nsplit == 1) {
+                ac_store4(a, ac_row(a, u, r, a.ld_out) + col, acc, l[r]);
+            } else {
+                w[r * HD + col] = acc.x;
+                w[r * HD + col + 1] = acc.y;
+                w[r * HD + col + 2] = acc.z;
+                w[r * HD + col + 3] = acc.w;
+                if (col == 0) {
+                    w[R * HD + r] = m[r];
+                    w[R * HD + R + r] = l[r];
+                }
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    }
+};
+
+// Starts the copies of steps into ring slots: called by a whole warp.
+template <int HD>
+struct AcCopies {
+    const KvLayer& c;
+    const AcUnit& u;
+    int maxlim, steps, lg16;
+    uint32_t ring;
+    float* scales;   // [4][2][4]: key and value scales of the four groups
+    __device__ __forceinline__ AcCopies(const KvLayer& c_, const AcUnit& u_, int maxlim_, int steps_, uint32_t ring_, float* scales_)
+        : c(c_), u(u_), maxlim(maxlim_), steps(steps_), lg16(c_.log_page - 4), ring(ring_), scales(scales_)
+    {
+    }
+
+    // The page of this lane's group (lane & 3) of a step; -1: not in the pool, -2: past the last key.
+    __device__ __forceinline__ int look(int step) const
+    {
+        const int g = 4 * step + (threadIdx.x & 3);
+        return step < steps && 16 * g < maxlim ? kv_page(c, u.b, g >> lg16) : -2;
+    }
+
+    // The keys (which = 0) or values of a step into slot s, and with the keys
+    // the groups' scales into [place], -0 standing for those of a group that
+    // cannot be read.  A slot's phase is lane 0's arrival with the byte count
+    // and one of each of lanes 0-7.
+    __device__ __forceinline__ void issue(int which, int step, int place, int s, uint32_t bar, int page) const
+    {
+        const int lane = threadIdx.x & 31, cc = lane & 3;
+        const unsigned valid = __ballot_sync(0xffffffffu, page >= 0) & 0xfu;
+        if (lane == 0) tc::mbar_arrive_expect_tx(bar, (uint32_t)__popc(valid) * 16u * HD);
+        __syncwarp();
+        if (lane < 8) {
+            const int64_t ph = (int64_t)page * c.heads + u.h;
+            if (lane < 4 && page >= 0)
+                tc::bulk_load(ring + s * 4 * ac_pitch(HD) + lane * ac_pitch(HD),
+                              (which ? c.v : c.k) + (ph << c.log_page) * HD + ((4 * step + cc) & ((1 << lg16) - 1)) * 16 * HD, 16u * HD, bar);
+            float* to = scales + place * 8 + lane;
+            if (which == 0 && page >= 0) {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(to)), "l"((lane < 4 ? c.ks : c.vs) + ph) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+            } else {
+                if (which == 0) *to = -0.0f;
+                tc::mbar_arrive(bar);
+            }
+            if (which == 0 && page == -1 && lane < 4) kv_flag(c.err, GBX_KV_BAD_PAGE);
+        }
+    }
+};
+
 // HD: head width; RT: 8-row tiles; W: warps; NS: slots of a warp's ring, each
 // the keys or the values of one step.
 template <int HD, int RT, int W, int NS>
@@ -400,7 +674,7 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
     __shared__ float s_scale[W][4][2][4];   // of step t in [t & 3]: key and value scales of the four groups
     __shared__ int s_abort;
     const KvLayer& c = a.c;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cc = lane & 3;
     uint32_t rank, csize;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
@@ -411,7 +685,6 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
     const AcUnit u = ac_unit(a, unit, R, &bad_len);
     if (bad_len && threadIdx.x == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
     if (u.rows <= 0) return;   // every CTA of the cluster alike
-    constexpr int hd = HD;
 
     // ---------------------------------------------------- this warp's ring
     // A slot: four groups of 16 hd bytes and 32 of padding (the groups' same
@@ -432,39 +705,10 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
     const int steps = (maxlim + kAcTile - 1) / kAcTile;
     const int stride = (int)csize * a.nsplit * W;
     const int first = (split * (int)csize + (int)rank) * W + warp;
-    const int lg16 = c.log_page - 4;
-    const int64_t page_bytes = (int64_t)hd << c.log_page;
-    // the page of this lane's group (lane & 3) of a step; -1: not in the pool, -2: past the last key
-    auto look = [&](int step) {
-        const int g = 4 * step + cc;
-        return step < steps && 16 * g < maxlim ? kv_page(c, u.b, g >> lg16) : -2;
-    };
-    // Starts the copies of this warp's k-th step's keys (which = 0) or values
-    // into slot s, and with the keys those of the groups' scales, -0 standing
-    // for the scales of a group that cannot be read.  A slot's phase is lane
-    // 0's arrival with the byte count and one of each of lanes 0-7.
-    auto issue = [&](int which, int k, int s, int page) {
-        const uint32_t bar = bar0 + 8 * s;
-        const unsigned valid = __ballot_sync(0xffffffffu, page >= 0) & 0xfu;
-        if (lane == 0) tc::mbar_arrive_expect_tx(bar, (uint32_t)__popc(valid) * 16u * (uint32_t)hd);
-        __syncwarp();
-        if (lane < 8) {
-            const int g = 4 * (first + k * stride) + cc;
-            const int64_t ph = (int64_t)page * c.heads + u.h;
-            if (lane < 4 && page >= 0)
-                tc::bulk_load(ring + s * slot_bytes + lane * pitch,
-                              (which ? c.v : c.k) + ph * page_bytes + (g & ((1 << lg16) - 1)) * 16 * hd, 16u * hd, bar);
-            float* to = &s_scale[warp][k & 3][lane >> 2][cc];
-            if (which == 0 && page >= 0) {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(to)), "l"((lane < 4 ? c.ks : c.vs) + ph) : "memory");
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-            } else {
-                if (which == 0) *to = -0.0f;
-                tc::mbar_arrive(bar);
-            }
-            if (which == 0 && page == -1 && lane < 4) kv_flag(c.err, GBX_KV_BAD_PAGE);
-        }
-    };
+    const AcCopies<HD> copies(c, u, maxlim, steps, ring, &s_scale[warp][0][0][0]);
+    // of this warp's k-th step
+    auto look = [&](int step) { return copies.look(step); };
+    auto issue = [&](int which, int k, int s, int page) { copies.issue(which, first + k * stride, k & 3, s, bar0 + 8 * s, page); };
 
     // pages of steps k + 1 and k + 2 of this warp while it works on step k
     static_assert(NS == 3 || NS == 4, "the page look-ahead below is two steps");
@@ -554,83 +798,145 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
         for (int rt = 0; rt < RT; ++rt) l[rt] = __int_as_float(0x7fc00000);
     }
 
-    // ---------------------------------------------------- the CTA's warps meet
+    // ---------------------------------------------------- the warps meet
     __syncthreads();   // the ring is done with
-    float* s_o = reinterpret_cast<float*>(ac_smem);   // [W][R][hd], then the CTA's own [R][hd]
-    float* s_m = s_o + (W + 1) * R * hd;              // [W][R], then the CTA's
-    float* s_l = s_m + (W + 1) * R;
-    const int nr = u.rows;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        l[rt] += __shfl_xor_sync(0xffffffffu, l[rt], 1);
-        l[rt] += __shfl_xor_sync(0xffffffffu, l[rt], 2);
-        const int r = 8 * rt + n;
-        if (r < nr) {
-            if (cc == 0) {
-                s_m[warp * R + r] = m[rt];
-                s_l[warp * R + r] = l[rt];
-            }
-#pragma unroll
-            for (int j = 0; j < HD / 8; ++j)
-                *reinterpret_cast<float2*>(s_o + (warp * R + r) * hd + 8 * j + 2 * cc) = o[rt][j];
+    AcMeet<HD, R, W> meet(ac_smem);
+    meet.put(warp, 0, u.rows, m, l, o);
+    __syncthreads();
+    meet.finish_few(a, u, unit, split, rank, csize, T);
+}
+
+// Many rows (the next tokens of a prompt): a CTA's W warps take 16 rows each and
+// go through the same steps, whose copies a warp of its own keeps in flight in
+// one ring.  The int8 tensor path bounds it: 16 rows x 64 tokens of width 64 are
+// 96 instructions of 8 cycles, and half as many exponentials as those take.
+template <int HD, int W, int NS>
+__global__ void __launch_bounds__(32 * (W + 1)) attn_cached_rows_kernel(const AcArgs a)
+{
+    grid_dependency_wait();
+    constexpr int RT = 2, R = 8 * RT * W, T = 32 * (W + 1);
+    static_assert(NS <= 6, "a step's scales are kept for four steps");
+    extern __shared__ __align__(128) uint8_t ac_smem[];
+    __shared__ uint64_t bars[2 * NS];
+    __shared__ float s_scale[4][2][4];
+    __shared__ int s_abort;
+    const KvLayer& c = a.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cc = lane & 3;
+    uint32_t rank, csize;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
+    const uint32_t cid = blockIdx.x >> (31 - __clz((int)csize));
+    const uint32_t unit = fast_div(cid, a.by_nsplit);
+    const int split = (int)(cid - unit * a.nsplit);
+    bool bad_len;
+    const AcUnit u = ac_unit(a, unit, R, &bad_len);
+    if (bad_len && threadIdx.x == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
+    if (u.rows <= 0) return;
+    constexpr int pitch = ac_pitch(HD), slot_bytes = 4 * pitch;
+    const uint32_t ring = tc::smem_u32(ac_smem), bar0 = tc::smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8 * s; };
+    auto empty = [&](int s) { return bar0 + 8 * (NS + s); };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            tc::mbar_init(full(s), 9);
+            tc::mbar_init(empty(s), W);
         }
+        s_abort = 0;
+        tc::fence_mbar_init();
     }
     __syncthreads();
-    const bool alone = csize == 1 && a.nsplit == 1;
-    for (int e = threadIdx.x; e < nr * hd; e += T) {
-        const int r = e / HD, col = e - r * HD;
-        float mx = -INFINITY;
+    volatile int* abort = &s_abort;
+    const int before = u.seq.len - u.seq.n + 1;
+    const int maxlim = before + (int)fast_div(u.r0 + u.rows - 1, a.by_g);   // keys the last row sees
+    const int steps = (maxlim + kAcTile - 1) / kAcTile;
+    const int stride = (int)csize * a.nsplit, first = split * (int)csize + (int)rank;
+
+    float2 o[RT][HD / 8];
+    float m[RT], l[RT];
 #pragma unroll
-        for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w * R + r]);
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        float acc = 0.0f, ll = 0.0f;
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = ac_exp2(s_m[w * R + r] - base);
-            acc += f * s_o[(w * R + r) * hd + col];
-            ll += f * s_l[w * R + r];
-        }
-        if (alone) {
-            ac_store(a, ac_row(a, u, r, a.ld_out) + col, ll == 0.0f ? 0.0f : acc / ll);
-        } else {
-            s_o[(W * R + r) * hd + col] = acc;
-            if (col == 0) {
-                s_m[W * R + r] = mx;
-                s_l[W * R + r] = ll;
+        for (int j = 0; j < HD / 8; ++j) o[rt][j] = make_float2(0.0f, 0.0f);
+    }
+    if (warp == W) {
+        // ------------------------------------------------ the copies
+        AcCopies<HD> copies(c, u, maxlim, steps, ring, &s_scale[0][0][0]);
+        int issued = 0, page = copies.look(first);
+        for (int step = first; step < steps; step += stride) {
+            const int next = copies.look(step + stride);
+            for (int which = 0; which < 2; ++which, ++issued) {
+                const int s = issued % NS;
+                if (issued >= NS && !tc::mbar_wait(empty(s), (issued / NS - 1) & 1, abort, kDeviceWaitNs)) goto stop;
+                copies.issue(which, step, (issued >> 1) & 3, s, full(s), page);
             }
+            page = next;
+        }
+    stop:
+        // every copy has landed before the CTA goes on
+        for (int j = max(0, issued - NS); j < issued; ++j) tc::mbar_wait(full(j % NS), (j / NS) & 1, nullptr, kDeviceWaitNs);
+    } else {
+        // ------------------------------------------------ this warp's rows
+        const int base = 8 * RT * warp;
+        AcDigits<RT, ac_chunks(HD)> q;
+        float qs[RT];
+        int limit[RT];
+        ac_queries<HD, RT>(a, u, base, q, qs, limit);
+        const int top = min(u.rows, base + 8 * RT) - 1;   // the warp's last row, if it has one
+        const int wmax = top < base ? 0 : before + (int)fast_div(u.r0 + top, a.by_g);
+        const int wmin = before + (int)fast_div(u.r0 + base, a.by_g);
+        const AcConst kc;
+        bool dead = false;
+        int k = 0, slot = 0;
+        uint32_t phase = 0;
+        uint64_t limit_ns = a.first_wait_ns;
+        auto leave = [&] {   // this warp has read the slot
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(empty(slot));
+            if (++slot == NS) {
+                slot = 0;
+                phase ^= 1;
+            }
+        };
+        for (int step = first; step < steps; step += stride, ++k) {
+            if (limit_ns == 0 || !tc::mbar_wait(full(slot), phase, abort, limit_ns)) {
+                dead = true;
+                break;
+            }
+            limit_ns = kDeviceWaitNs;
+            const int t0 = step * kAcTile;
+            const bool some = t0 < wmax;   // a step past the warp's last key is let go by
+            AcDigits<RT, 2> p;
+            float alpha[RT], beta[RT];
+            if (some) {
+                const float ks = s_scale[k & 3][0][cc], vs = s_scale[k & 3][1][cc];
+                const bool seen = !(ks == 0.0f && signbit(ks));
+                const bool edge = __any_sync(0xffffffffu, !seen) || t0 + kAcTile > wmin;
+                const uint32_t kb = ring + slot * slot_bytes;
+                if (edge) ac_scores<HD, RT>(kb, t0, seen, true, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+                else ac_scores<HD, RT>(kb, t0, true, false, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+            }
+            leave();
+            if (!tc::mbar_wait(full(slot), phase, abort, kDeviceWaitNs)) {
+                dead = true;
+                break;
+            }
+            if (some) ac_values<HD, RT>(ring + slot * slot_bytes, p, alpha, beta, o, kc);
+            leave();
+        }
+        if (dead) {
+            *abort = 1;
+            if (lane == 0) kv_flag(c.err, GBX_LINEAR_TIMEOUT);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) l[rt] = __int_as_float(0x7fc00000);
         }
     }
-    if (alone) return;
-    // ---------------------------------------------------- the cluster's CTAs meet
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-    auto peer = [&](uint32_t p, const float* x) -> float {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(tc::mapa(tc::smem_u32(x), p)) : "memory");
-        return v;
-    };
-    for (int e = (int)rank * T + threadIdx.x; e < nr * hd; e += (int)csize * T) {
-        const int r = e / HD, col = e - r * HD;
-        float mx = -INFINITY;
-        for (uint32_t p = 0; p < csize; ++p) mx = fmaxf(mx, peer(p, s_m + W * R + r));
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        float acc = 0.0f, ll = 0.0f;
-        for (uint32_t p = 0; p < csize; ++p) {
-            const float f = ac_exp2(peer(p, s_m + W * R + r) - base);
-            acc += f * peer(p, s_o + (W * R + r) * hd + col);
-            ll += f * peer(p, s_l + W * R + r);
-        }
-        if (a.nsplit == 1) {
-            ac_store(a, ac_row(a, u, r, a.ld_out) + col, ll == 0.0f ? 0.0f : acc / ll);
-        } else {
-            float* w = a.ws + ((int64_t)unit * a.nsplit + split) * (R * (hd + 2));
-            w[r * hd + col] = acc;
-            if (col == 0) {
-                w[R * hd + r] = mx;
-                w[R * hd + R + r] = ll;
-            }
-        }
-    }
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    __syncthreads();   // the ring is done with
+    AcMeet<HD, R, 1> meet(ac_smem);
+    if (warp < W) meet.put(0, 8 * RT * warp, u.rows, m, l, o);
+    __syncthreads();
+    meet.finish(a, u, unit, split, rank, csize, T);
 }
 
 // Joins the nsplit partial results of each unit: one CTA per unit.
@@ -665,6 +971,7 @@ __global__ void __launch_bounds__(256) attn_cached_join_kernel(const AcArgs a, i
 // 275 with 2 and 4, 290 with 4 and 4, 339 with 1 and 4; at 2 x 8 heads x 120,001
 // tokens of width 128: 93 with 4 and 3, 101 with 3 and 3, 103 with 2 and 3.
 constexpr int kAcWarps = 4, kAcSlots = 3;
+constexpr int kAcRowWarps = 4, kAcRowSlots = 6;
 
 constexpr int kAcSmemPerSM = 228 * 1024;
 
@@ -679,8 +986,11 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, Ac
     if (device_info(&di) != GBX_OK) return GBX_ECUDA;
     const int G = H / c->heads;
     const int64_t rows = (int64_t)S * G;
-    p->rt = rows > 8 ? 2 : 1;
-    const int R = 8 * p->rt, W = kAcWarps, NS = kAcSlots;
+    // 8 or 16 rows that the warps share, splitting the steps; from 17 on 64 rows that
+    // split the warps, going through the steps together
+    p->rt = rows <= 8 ? 1 : rows <= 16 ? 2 : 8;
+    const bool many = p->rt == 8;
+    const int R = 8 * p->rt, W = many ? 1 : kAcWarps;   // warps that split the steps
     const int64_t nrb = (rows + R - 1) / R;
     p->units = (int64_t)B * c->heads * nrb;
     if (nrb > 0x7fffffff || p->units * kAcMaxCluster > 0x7fffffffLL)
@@ -692,7 +1002,8 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, Ac
     // the workspace, which costs a second launch and is taken where it at least
     // doubles the CTAs.
     const int64_t steps = ((int64_t)max_pages * c->page + kAcTile - 1) / kAcTile;
-    const int64_t resident = (int64_t)di.sm_count * (int64_t)((size_t)kAcSmemPerSM / (W * NS * 4 * ac_pitch(c->hd) + 2048));
+    const int64_t per_sm = many ? (c->hd <= 64 ? 3 : c->hd <= 96 ? 2 : 1) : (int64_t)((size_t)kAcSmemPerSM / (kAcWarps * kAcSlots * 4 * ac_pitch(c->hd) + 2048));
+    const int64_t resident = di.sm_count * per_sm;
     int64_t share = resident / p->units;
     if (share > (steps + W - 1) / W) share = (steps + W - 1) / W;
     p->csize = 1;
@@ -716,16 +1027,19 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, Ac
 template <int HD, int RT>
 static int ac_launch(const AcArgs& a, const AcPlan& p, cudaStream_t s)
 {
-    constexpr int R = 8 * RT, W = kAcWarps, NS = kAcSlots;
-    auto k = attn_cached_kernel<HD, RT, W, NS>;
-    const size_t ring = (size_t)W * NS * 4 * ac_pitch(HD);
-    const size_t meet = sizeof(float) * (size_t)(W + 1) * R * (a.c.hd + 2);
+    constexpr bool many = RT == 8;
+    constexpr int R = 8 * RT;
+    void (*k)(AcArgs);
+    if constexpr (many) k = attn_cached_rows_kernel<HD, kAcRowWarps, kAcRowSlots>;
+    else k = attn_cached_kernel<HD, RT, kAcWarps, kAcSlots>;
+    const size_t ring = (size_t)(many ? kAcRowSlots : kAcWarps * kAcSlots) * 4 * ac_pitch(HD);
+    const size_t meet = sizeof(float) * (size_t)((many ? 1 : kAcWarps) + 1) * R * (HD + 2);
     const size_t smem = ring > meet ? ring : meet;
     if (smem > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return check_launch("gbx_attn_cached: shared-memory attribute");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.units * p.nsplit * p.csize));
-    cfg.blockDim = dim3(32 * W);
+    cfg.blockDim = dim3(32 * (many ? kAcRowWarps + 1 : kAcWarps));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -808,12 +1122,13 @@ extern "C" int gbx_attn_cached(const gbx_kv_cache* cache_host, int layer, const 
     a.by_g = make_fastdiv(a.G);
     a.by_nsplit = make_fastdiv(p.nsplit);
     a.by_hd = make_fastdiv(a.c.hd);
+    a.vec_out = aligned16(out) && aligned16(out_lo) && ld_out % 4 == 0;
     a.vec = aligned16(q_hi) && aligned16(q_lo) && ld % 4 == 0;
     a.first_wait_ns = first_wait_limit_ns();
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     auto launch = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        return p.rt == 1 ? ac_launch<HD, 1>(a, p, s) : ac_launch<HD, 2>(a, p, s);
+        return p.rt == 1 ? ac_launch<HD, 1>(a, p, s) : p.rt == 2 ? ac_launch<HD, 2>(a, p, s) : ac_launch<HD, 8>(a, p, s);
     };
     switch (a.c.hd) {
     case 16: return launch(std::integral_constant<int, 16>());
