@@ -21,6 +21,24 @@ struct gbx_sharded {
     gbx::ShardedModel model;
 };
 
+struct gbx_session {
+    gbx::Session session;
+    int vocab;
+};
+
+// No exception leaves a C entry point: an allocation that fails is an error code.
+template <class F>
+static int guarded(const char* what, F f)
+{
+    try {
+        return f();
+    } catch (const std::bad_alloc&) {
+        return gbx::set_error(GBX_ENOMEM, "%s: out of memory", what);
+    } catch (...) {
+        return gbx::set_error(GBX_EINVAL, "%s: unexpected failure", what);
+    }
+}
+
 extern "C" {
 
 gbx_gguf* gbx_gguf_open(const char* path)
@@ -198,6 +216,130 @@ int gbx_sharded_forward(gbx_sharded* s, const int32_t* ids_host, int64_t n_ids, 
     if (out.empty()) return gbx::set_error(GBX_EINVAL, "%s", s->model.lastError().c_str());
     std::memcpy(logits_host, out.data(), out.size() * sizeof(float));
     return GBX_OK;
+}
+
+gbx_session* gbx_session_open(gbx_model* m, int64_t pages, int page_size)
+{
+    if (!m) {
+        gbx::set_error(GBX_EINVAL, "gbx_session_open: null model");
+        return nullptr;
+    }
+    if (pages <= 0 || pages > 0x7fffffffLL) {
+        gbx::set_error(GBX_EINVAL, "gbx_session_open: %lld pages", (long long)pages);
+        return nullptr;
+    }
+    gbx_session* s = nullptr;
+    const int rc = guarded("gbx_session_open", [&] {
+        s = new gbx_session{{m->model, pages, page_size}, m->model.getVocabSize()};
+        return GBX_OK;
+    });
+    if (rc == GBX_OK && !s->session.ok()) {
+        gbx::set_error(GBX_EINVAL, "%s", s->session.lastError().c_str());
+        delete s;
+        return nullptr;
+    }
+    return rc == GBX_OK ? s : nullptr;
+}
+
+void gbx_session_close(gbx_session* s) { delete s; }
+
+int gbx_session_new(gbx_session* s)
+{
+    if (!s) return gbx::set_error(GBX_EINVAL, "gbx_session_new: null session"), -1;
+    int id = -1;
+    guarded("gbx_session_new", [&] { return id = s->session.newSequence(), GBX_OK; });
+    return id;
+}
+
+int gbx_session_fork(gbx_session* s, int seq)
+{
+    if (!s) return gbx::set_error(GBX_EINVAL, "gbx_session_fork: null session"), -1;
+    int id = -1;
+    const int rc = guarded("gbx_session_fork", [&] { return id = s->session.fork(seq), GBX_OK; });
+    if (rc == GBX_OK && id < 0) gbx::set_error(GBX_EINVAL, "gbx_session_fork: no sequence %d", seq);
+    return id;
+}
+
+int gbx_session_truncate(gbx_session* s, int seq, int64_t length)
+{
+    if (!s) return gbx::set_error(GBX_EINVAL, "gbx_session_truncate: null session");
+    return guarded("gbx_session_truncate", [&] {
+        return s->session.truncate(seq, length)
+                   ? (int)GBX_OK
+                   : gbx::set_error(GBX_EINVAL, "gbx_session_truncate: sequence %d to %lld tokens", seq, (long long)length);
+    });
+}
+
+int gbx_session_release(gbx_session* s, int seq)
+{
+    if (!s) return gbx::set_error(GBX_EINVAL, "gbx_session_release: null session");
+    return guarded("gbx_session_release", [&] {
+        return s->session.release(seq) ? (int)GBX_OK : gbx::set_error(GBX_EINVAL, "gbx_session_release: no sequence %d", seq);
+    });
+}
+
+int64_t gbx_session_compact(gbx_session* s)
+{
+    if (!s) return gbx::set_error(GBX_EINVAL, "gbx_session_compact: null session"), -1;
+    int64_t n = -1;
+    const int rc = guarded("gbx_session_compact", [&] { return n = s->session.compact(), GBX_OK; });
+    if (rc == GBX_OK && n < 0) gbx::set_error(GBX_ECUDA, "%s", s->session.lastError().c_str());
+    return n;
+}
+
+int64_t gbx_session_length(gbx_session* s, int seq) { return s ? s->session.length(seq) : -1; }
+
+int64_t gbx_session_free_pages(gbx_session* s) { return s ? s->session.freePages() : -1; }
+
+int gbx_session_forward(gbx_session* s, const int32_t* seqs_host, int n_seq, const int32_t* ids_host, int64_t n_ids,
+                        const int32_t* counts_host, int all_rows, float* logits_host)
+{
+    if (!s || !seqs_host || !ids_host || !counts_host || !logits_host || n_seq <= 0 || n_ids <= 0)
+        return gbx::set_error(GBX_EINVAL, "gbx_session_forward: bad argument");
+    return guarded("gbx_session_forward", [&] {
+        const std::vector<float> out = s->session.forward({seqs_host, seqs_host + n_seq}, {ids_host, ids_host + n_ids},
+                                                          {counts_host, counts_host + n_seq}, all_rows != 0);
+        if (out.empty()) return gbx::set_error(GBX_EINVAL, "%s", s->session.lastError().c_str());
+        std::memcpy(logits_host, out.data(), out.size() * sizeof(float));
+        return (int)GBX_OK;
+    });
+}
+
+int gbx_session_next_tokens(gbx_session* s, const int32_t* seqs_host, int n_seq, const int32_t* ids_host, int64_t n_ids,
+                            const int32_t* counts_host, double temperature, const double* u_host, int32_t* out_ids_host)
+{
+    if (!s || !seqs_host || !ids_host || !counts_host || !out_ids_host || n_seq <= 0 || n_ids <= 0)
+        return gbx::set_error(GBX_EINVAL, "gbx_session_next_tokens: bad argument");
+    return guarded("gbx_session_next_tokens", [&] {
+        std::vector<double> u;
+        if (u_host) u.assign(u_host, u_host + n_seq);
+        const std::vector<int> out = s->session.nextTokens({seqs_host, seqs_host + n_seq}, {ids_host, ids_host + n_ids},
+                                                           {counts_host, counts_host + n_seq}, temperature, u);
+        if (out.empty()) return gbx::set_error(GBX_EINVAL, "%s", s->session.lastError().c_str());
+        for (int i = 0; i < n_seq; ++i) out_ids_host[i] = out[i];
+        return (int)GBX_OK;
+    });
+}
+
+int gbx_session_verify(gbx_session* s, const int32_t* seqs_host, int n_seq, const int32_t* ids_host, int n_draft,
+                       const int32_t* draft_len_host, const float* draft_logits_host, double temperature,
+                       const double* u_host, int32_t* out_ids_host, int32_t* n_accepted_host)
+{
+    if (!s || !seqs_host || !ids_host || !out_ids_host || !n_accepted_host || n_seq <= 0 || n_draft < 0 || n_draft > 256)
+        return gbx::set_error(GBX_EINVAL, "gbx_session_verify: bad argument");
+    return guarded("gbx_session_verify", [&] {
+        const size_t rows = (size_t)n_seq * (n_draft + 1);
+        std::vector<double> u;
+        if (u_host) u.assign(u_host, u_host + rows);
+        std::vector<int> lens, out, acc;
+        if (draft_len_host) lens.assign(draft_len_host, draft_len_host + n_seq);
+        if (!s->session.verify({seqs_host, seqs_host + n_seq}, {ids_host, ids_host + rows}, n_draft, lens, draft_logits_host,
+                               temperature, u, &out, &acc))
+            return gbx::set_error(GBX_EINVAL, "%s", s->session.lastError().c_str());
+        for (size_t i = 0; i < rows; ++i) out_ids_host[i] = out[i];
+        for (int i = 0; i < n_seq; ++i) n_accepted_host[i] = acc[i];
+        return (int)GBX_OK;
+    });
 }
 
 }  // extern "C"

@@ -268,7 +268,7 @@ bool TransformerModel::loadModel(const std::string& ggufPath)
     return true;
 }
 
-bool TransformerModel::ensureBuffers(int64_t tokens, int seq)
+bool TransformerModel::ensureBuffers(int64_t tokens, int seq, const CachedStep* step)
 {
     Impl& m = *impl_;
     const int64_t d = embedDim_, F = ffnDim_, B = tokens / seq;
@@ -276,10 +276,11 @@ bool TransformerModel::ensureBuffers(int64_t tokens, int seq)
     int64_t G = kScoreGroupFloats / per_seq;
     G = G < 1 ? 1 : (G > B ? B : G);
     m.score_group = (int)G;
-    // the fused attention needs no score buffers
+    // the fused attention needs no score buffers, the cached one neither
     m.fused = m.want_fused && headDim_ == 64 && d % 4 == 0;
-    const int64_t score_floats = m.fused ? 1 : G * per_seq;
-    const int64_t vt_floats = m.fused ? 1 : G * seq * d;
+    const int64_t score_floats = m.fused || step ? 1 : G * per_seq;
+    const int64_t vt_floats = m.fused || step ? 1 : G * seq * d;
+    const int64_t rows = step && step->allRows ? tokens : B;   // of logits
     // the largest split-K workspace of the four contractions
     size_t ws = 1;
     const int64_t shapes[4][2] = {{3 * d, d}, {d, d}, {F, d}, {d, F}};
@@ -293,8 +294,8 @@ bool TransformerModel::ensureBuffers(int64_t tokens, int seq)
                     m.vt.ensure((size_t)vt_floats) && m.vt_lo.ensure((size_t)vt_floats) &&
                     m.attn.ensure(tokens * d) && m.attn_lo.ensure(tokens * d) && m.up.ensure(tokens * F) &&
                     m.up_lo.ensure(tokens * F) && m.splitk_ws.ensure(ws) &&
-                    m.last_y.ensure(B * d) &&
-                    m.logits.ensure((size_t)B * vocab_);
+                    m.last_y.ensure(rows * d) &&
+                    m.logits.ensure((size_t)rows * vocab_);
     if (!ok) return fail("cudaMalloc of activation buffers failed");
     if ((size_t)tokens > m.ids_n) {
         if (m.ids) cudaFree(m.ids);
@@ -370,6 +371,15 @@ int TransformerModel::nextTokenWithDraw(const std::vector<int>& tokenIDs, double
     return selected;
 }
 
+bool TransformerModel::streamAndDevice(gbx_stream_t* stream, int* device) const
+{
+    *stream = reinterpret_cast<gbx_stream_t>(impl_->stream);
+    *device = impl_->device;
+    return impl_->stream != nullptr;
+}
+
+const float* TransformerModel::deviceLogits() const { return impl_->logits.p; }
+
 void TransformerModel::setFusedAttention(bool on) { impl_->want_fused = on; }
 
 bool TransformerModel::fusedAttention() const { return impl_->want_fused; }
@@ -389,7 +399,7 @@ std::vector<float> TransformerModel::forwardHidden(const std::vector<int>& token
     return hidden;
 }
 
-bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, float* hidden_host)
+bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, float* hidden_host, const CachedStep* step)
 {
     Impl& m = *impl_;
     err_.clear();
@@ -404,7 +414,7 @@ bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, f
     for (int id : tokenIDs)
         if (id < 0 || id >= vocab_) return fail("forward: token id " + std::to_string(id) + " outside the token table");
     cudaSetDevice(m.device);
-    if (!ensureBuffers(N, S)) return false;
+    if (!ensureBuffers(N, S, step)) return false;
 
     const int d = embedDim_, H = numHeads_, hd = headDim_, F = ffnDim_, V = vocab_;
     cudaStream_t st = m.stream;
@@ -430,7 +440,7 @@ bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, f
         cudaMemsetAsync(m.err, 0, sizeof(int32_t), st) != cudaSuccess)
         return fail("host-to-device copy of token ids failed");
     // the embedding and layer 0's attention LayerNorm in one pass (h written once, not re-read)
-    check(gbx_embed_layernorm(m.ids, m.wte, m.wte_dt, m.wpe, m.wpe_dt, nullptr, m.h.p, m.ln.p, m.ln_lo.p,
+    check(gbx_embed_layernorm(m.ids, m.wte, m.wte_dt, m.wpe, m.wpe_dt, step ? step->posIds : nullptr, m.h.p, m.ln.p, m.ln_lo.p,
                               numLayers_ > 0 ? m.layers[0].ln1_g : nullptr, numLayers_ > 0 ? m.layers[0].ln1_b : nullptr,
                               N, S, 0, d, V, nCtx_, 1e-5f, m.err, gs));
     // forwardHidden: the residual stream after the embedding and after each layer
@@ -448,13 +458,21 @@ bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, f
         const Impl::LayerW& W = m.wpairs[l];
         if (l > 0) check(gbx_layernorm_pair(m.h.p, m.ln.p, m.ln_lo.p, L.ln1_g, L.ln1_b, N, d, 1e-5f, gs));
         linear(m.ln.p, m.ln_lo.p, W.qkv, L.qkv_b, nullptr, m.qkv.p, m.qkv_lo.p, N, 3 * d, d, GBX_ACT_NONE);
-        if (m.fused) {
+        if (step)
+            check(gbx_kv_append(step->cache, l, step->table, step->maxPages, step->kvLen, step->nNew, batch, S, m.qkv.p + d,
+                                m.qkv_lo.p + d, m.qkv.p + 2 * d, m.qkv_lo.p + 2 * d, 3 * d, m.err, gs));
+        if (step && !(step->fresh && m.fused)) {
+            // the new rows over everything cached, their own keys and values included
+            check(gbx_attn_cached(step->cache, l, m.qkv.p, m.qkv_lo.p, 3 * d, step->table, step->maxPages, step->kvLen,
+                                  step->nNew, batch, S, H, scale, m.attn.p, m.attn_lo.p, d, step->workspace,
+                                  step->workspaceFloats, m.err, gs));
+        } else if (m.fused) {
             // attn = softmax(mask(Q K^T / sqrt(hd))) V for every head of every
             // sequence in one launch, as a tf32 pair
             check(gbx_attn_fused(m.qkv.p, m.qkv_lo.p, m.qkv.p + d, m.qkv_lo.p + d, 3 * d, m.qkv.p + 2 * d,
                                  m.qkv_lo.p + 2 * d, m.attn.p, m.attn_lo.p, d, batch, S, H, hd, scale, 1, m.err, gs));
         }
-        for (int b0 = 0; !m.fused && b0 < batch; b0 += m.score_group) {
+        for (int b0 = 0; !m.fused && !step && b0 < batch; b0 += m.score_group) {
             const int g = batch - b0 < m.score_group ? batch - b0 : m.score_group;
             const float* qh = m.qkv.p + (int64_t)b0 * S * 3 * d;
             const float* ql = m.qkv_lo.p + (int64_t)b0 * S * 3 * d;
@@ -474,7 +492,16 @@ bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, f
         linear(m.up.p, m.up_lo.p, W.down, L.down_b, m.h.p, m.h.p, nullptr, N, d, F, GBX_ACT_NONE);
         keep_hidden(l + 1);
     }
-    if (rc == GBX_OK) {
+    if (rc == GBX_OK && step && step->allRows) {
+        check(gbx_layernorm(m.h.p, m.last_y.p, m.lnf_g, m.lnf_b, N, d, 1e-5f, gs));
+        check(gbx_logits(m.last_y.p, N, m.wte, m.wte_dt, m.logits.p, V, d, gs));
+    } else if (rc == GBX_OK && step && !step->even) {
+        // sequences of different counts end in different rows
+        for (int b = 0; b < batch; ++b)
+            check(gbx_layernorm(m.h.p + ((int64_t)b * S + step->counts[b] - 1) * d, m.last_y.p + (int64_t)b * d, m.lnf_g, m.lnf_b,
+                                1, d, 1e-5f, gs));
+        check(gbx_logits(m.last_y.p, batch, m.wte, m.wte_dt, m.logits.p, V, d, gs));
+    } else if (rc == GBX_OK) {
         // ln_f of each sequence's last row of h (transformer.cu:883-896)
         check(gbx_final_layernorm(nullptr, m.h.p, m.last_y.p, m.lnf_g, m.lnf_b, batch, S, d, 1e-5f, gs));
         check(gbx_logits(m.last_y.p, batch, m.wte, m.wte_dt, m.logits.p, V, d, gs));
@@ -488,6 +515,7 @@ bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, f
     if (err_host & GBX_LINEAR_TIMEOUT)
         return fail("a device wait timed out (a tensor-core contraction or the staged embedding): the forward's "
                     "outputs are incomplete");
+    if (err_host & (GBX_KV_BAD_PAGE | GBX_KV_BAD_LEN)) return fail("the cache reported a page or a length out of range");
     if (err_host) return fail("embedding reported out-of-range ids or positions");
     return true;
 }

@@ -8,7 +8,8 @@
 getTensorGPU and ``tensor_gpu_raw`` gives the tensor's GGUF bytes on the
 device.  ``Model`` mirrors TransformerModel (transformer.cu:744-1051):
 ``forward(ids)`` returns the last token's logits; ``forward(ids, batch=B)``
-runs B equal-length sequences and returns [B, vocab].
+runs B equal-length sequences and returns [B, vocab].  ``Session`` (no
+counterpart in the reference) generates over a paged 8-bit key/value cache.
 
 There is no fallback: importing fails loudly when the library is missing.
 """
@@ -44,6 +45,18 @@ SIGNATURES = {
     "gbx_model_forward_hidden": ([_vp, _vp, _i64, _int, _vp, _i64], _int),
     "gbx_model_set_fused_attention": ([_vp, _int], _int),
     "gbx_model_next_token": ([_vp, _vp, _i64, ctypes.c_double, ctypes.c_double, _vp, _vp, _vp], _int),
+    "gbx_session_open": ([_vp, _i64, _int], _vp),
+    "gbx_session_close": ([_vp], None),
+    "gbx_session_new": ([_vp], _int),
+    "gbx_session_fork": ([_vp, _int], _int),
+    "gbx_session_truncate": ([_vp, _int, _i64], _int),
+    "gbx_session_release": ([_vp, _int], _int),
+    "gbx_session_compact": ([_vp], _i64),
+    "gbx_session_length": ([_vp, _int], _i64),
+    "gbx_session_free_pages": ([_vp], _i64),
+    "gbx_session_forward": ([_vp, _vp, _int, _vp, _i64, _vp, _int, _vp], _int),
+    "gbx_session_next_tokens": ([_vp, _vp, _int, _vp, _i64, _vp, ctypes.c_double, _vp, _vp], _int),
+    "gbx_session_verify": ([_vp, _vp, _int, _vp, _int, _vp, _vp, ctypes.c_double, _vp, _vp, _vp], _int),
     "gbx_sharded_open": ([_cp, _vp, _int], _vp),
     "gbx_sharded_close": ([_vp], None),
     "gbx_sharded_forward": ([_vp, _vp, _i64, _int, _vp], _int),
@@ -220,3 +233,128 @@ class ShardedModel:
         if rc != 0:
             raise _err(rc)
         return out
+
+
+class Session:
+    """Cached generation over a Model (gbx::Session): sequences in a paged 8-bit
+    key/value cache of `pages` pages of `page_size` tokens; a step costs its
+    new tokens only."""
+
+    def __init__(self, model: Model, pages: int, page_size: int = 64):
+        self.model = model   # outlives the session
+        self.vocab = model.config["vocab"]
+        self.h = lib().gbx_session_open(model.h, pages, page_size)
+        if not self.h:
+            raise _err()
+
+    def close(self):
+        if self.h:
+            lib().gbx_session_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def new(self) -> int:
+        """An empty sequence."""
+        seq = lib().gbx_session_new(self.h)
+        if seq < 0:
+            raise _err(1)
+        return seq
+
+    def fork(self, seq: int) -> int:
+        """A sequence that continues from where `seq` stands (its pages are shared until written to)."""
+        new = lib().gbx_session_fork(self.h, seq)
+        if new < 0:
+            raise _err(1)
+        return new
+
+    def truncate(self, seq: int, length: int):
+        rc = lib().gbx_session_truncate(self.h, seq, length)
+        if rc:
+            raise _err(rc)
+
+    def release(self, seq: int):
+        rc = lib().gbx_session_release(self.h, seq)
+        if rc:
+            raise _err(rc)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the lowest places; how many moved."""
+        n = lib().gbx_session_compact(self.h)
+        if n < 0:
+            raise _err(4)
+        return n
+
+    def length(self, seq: int) -> int:
+        return lib().gbx_session_length(self.h, seq)
+
+    def free_pages(self) -> int:
+        return lib().gbx_session_free_pages(self.h)
+
+    @staticmethod
+    def _rows(seqs, tokens):
+        """seqs, ids (one sequence after another) and counts as int32 arrays."""
+        seqs = np.ascontiguousarray(seqs, dtype=np.int32).ravel()
+        rows = [np.ascontiguousarray(t, dtype=np.int32).ravel() for t in tokens]
+        if len(rows) != seqs.size:
+            raise ValueError(f"{len(rows)} token lists for {seqs.size} sequences")
+        counts = np.array([r.size for r in rows], dtype=np.int32)
+        return seqs, np.ascontiguousarray(np.concatenate(rows)) if rows else np.zeros(0, np.int32), counts
+
+    def forward(self, seqs, tokens, all_rows: bool = False) -> np.ndarray:
+        """Appends tokens[i] (ids) to sequence seqs[i]; logits [n, vocab] of each
+        sequence's last token, or of every token in order."""
+        seqs, ids, counts = self._rows(seqs, tokens)
+        out = np.empty((ids.size if all_rows else seqs.size, self.vocab), dtype=np.float32)
+        rc = lib().gbx_session_forward(self.h, _np_ptr(seqs), seqs.size, _np_ptr(ids), ids.size, _np_ptr(counts),
+                                       1 if all_rows else 0, _np_ptr(out))
+        if rc != 0:
+            raise _err(rc)
+        return out
+
+    def next_tokens(self, seqs, tokens, temperature=0.0, u=None) -> np.ndarray:
+        """forward, and each sequence's next token (the reference's rule; u: a draw in [0, 1) each)."""
+        seqs, ids, counts = self._rows(seqs, tokens)
+        out = np.empty(seqs.size, dtype=np.int32)
+        u = None if u is None else np.ascontiguousarray(u, dtype=np.float64).ravel()
+        if u is not None and u.size != seqs.size:
+            raise ValueError("a draw for each sequence")
+        rc = lib().gbx_session_next_tokens(self.h, _np_ptr(seqs), seqs.size, _np_ptr(ids), ids.size, _np_ptr(counts),
+                                           float(temperature), None if u is None else _np_ptr(u), _np_ptr(out))
+        if rc != 0:
+            raise _err(rc)
+        return out
+
+    def verify(self, seqs, tokens, temperature=0.0, u=None, draft_logits=None, draft_len=None):
+        """One speculative step.  tokens [n, k + 1]: each sequence's pending token
+        and k drafts; returns (ids [n, k + 1]: the accepted drafts, the next
+        token, -1s; accepted [n])."""
+        seqs = np.ascontiguousarray(seqs, dtype=np.int32).ravel()
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        if tokens.ndim != 2 or tokens.shape[0] != seqs.size or tokens.shape[1] < 1:
+            raise ValueError("tokens must be [sequences, drafts + 1]")
+        k = tokens.shape[1] - 1
+        u = None if u is None else np.ascontiguousarray(u, dtype=np.float64)
+        if u is not None and u.shape != tokens.shape:
+            raise ValueError("u must have the shape of tokens")
+        if draft_logits is not None:
+            draft_logits = np.ascontiguousarray(draft_logits, dtype=np.float32)
+            if draft_logits.shape != (seqs.size, k, self.vocab):
+                raise ValueError("draft_logits must be [sequences, drafts, vocab]")
+        if draft_len is not None:
+            draft_len = np.ascontiguousarray(draft_len, dtype=np.int32).ravel()
+            if draft_len.size != seqs.size:
+                raise ValueError("a draft count for each sequence")
+        out = np.empty(tokens.shape, dtype=np.int32)
+        acc = np.empty(seqs.size, dtype=np.int32)
+        rc = lib().gbx_session_verify(self.h, _np_ptr(seqs), seqs.size, _np_ptr(tokens), k,
+                                      None if draft_len is None else _np_ptr(draft_len),
+                                      None if draft_logits is None else _np_ptr(draft_logits), float(temperature),
+                                      None if u is None else _np_ptr(u), _np_ptr(out), _np_ptr(acc))
+        if rc != 0:
+            raise _err(rc)
+        return out, acc

@@ -19,6 +19,7 @@ extern "C" {
 typedef struct gbx_gguf gbx_gguf;
 typedef struct gbx_model gbx_model;
 typedef struct gbx_sharded gbx_sharded;
+typedef struct gbx_session gbx_session;
 
 /* GGUFLoader::loadFromFile (transformer.cu:657-674). */
 gbx_gguf* gbx_gguf_open(const char* path);
@@ -77,6 +78,42 @@ int gbx_model_next_token(gbx_model* m, const int32_t* ids_host, int64_t n_ids, d
 gbx_sharded* gbx_sharded_open(const char* gguf_path, const int32_t* devices, int n);
 void gbx_sharded_close(gbx_sharded* s);
 int gbx_sharded_forward(gbx_sharded* s, const int32_t* ids_host, int64_t n_ids, int batch, float* logits_host);
+
+/* Session (gbx_model.hpp): cached generation over a paged 8-bit key/value cache
+ * of `pages` pages of `page_size` tokens (16, 32, 64 or 128) for all layers.  No
+ * counterpart in the reference.  The model must outlive the session; the two
+ * are used by one thread at a time.  Sequences are named by the numbers that
+ * gbx_session_new and gbx_session_fork return (negative: none). */
+gbx_session* gbx_session_open(gbx_model* m, int64_t pages, int page_size);
+void gbx_session_close(gbx_session* s);
+int gbx_session_new(gbx_session* s);
+int gbx_session_fork(gbx_session* s, int seq);
+int gbx_session_truncate(gbx_session* s, int seq, int64_t length);
+int gbx_session_release(gbx_session* s, int seq);
+/* Pages moved to the lowest places, or -1. */
+int64_t gbx_session_compact(gbx_session* s);
+int64_t gbx_session_length(gbx_session* s, int seq);
+int64_t gbx_session_free_pages(gbx_session* s);
+/* Appends counts[i] tokens to sequence seqs[i] (ids: n_ids of them, one sequence
+ * after another); logits_host receives vocab floats for each sequence's last
+ * token, or with all_rows != 0 for every token.  On failure every sequence
+ * keeps the length it had. */
+int gbx_session_forward(gbx_session* s, const int32_t* seqs_host, int n_seq, const int32_t* ids_host, int64_t n_ids,
+                        const int32_t* counts_host, int all_rows, float* logits_host);
+/* The same, and each sequence's next token (gbx_select_tokens) with the draws
+ * u_host (n_seq of them; may be NULL at temperature <= 0.01). */
+int gbx_session_next_tokens(gbx_session* s, const int32_t* seqs_host, int n_seq, const int32_t* ids_host, int64_t n_ids,
+                            const int32_t* counts_host, double temperature, const double* u_host, int32_t* out_ids_host);
+/* One speculative step (gbx_verify_tokens): ids_host [n_seq][n_draft + 1] are
+ * each sequence's pending token and its drafts, draft_len_host (may be NULL)
+ * how many of them count, draft_logits_host [n_seq][n_draft][vocab] (may be
+ * NULL), u_host [n_seq][n_draft + 1] (may be NULL at temperature <= 0.01).
+ * out_ids_host [n_seq][n_draft + 1]: the accepted drafts, the next token, -1s;
+ * n_accepted_host [n_seq].  The pending token and the accepted drafts stay in
+ * the cache. */
+int gbx_session_verify(gbx_session* s, const int32_t* seqs_host, int n_seq, const int32_t* ids_host, int n_draft,
+                       const int32_t* draft_len_host, const float* draft_logits_host, double temperature,
+                       const double* u_host, int32_t* out_ids_host, int32_t* n_accepted_host);
 
 #ifdef __cplusplus
 }

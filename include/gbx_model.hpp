@@ -51,6 +51,8 @@
 //     sm_100a kernels behind gbx.h.  Loading keeps a tf32 pair of every f32
 //     weight matrix on the device (two extra fp32 copies); f16 / bf16
 //     weights need none.
+//   - Session (new) generates over a paged key/value cache: the reference's
+//     generate runs the whole prefix again for every token (:986-1036).
 #pragma once
 
 #include <cstdint>
@@ -188,9 +190,134 @@ private:
     int embedDim_ = 0, numHeads_ = 0, headDim_ = 0, numLayers_ = 0, ffnDim_ = 0, vocab_ = 0, nCtx_ = 0;
     std::string err_;
     bool fail(const std::string& msg);
-    bool ensureBuffers(int64_t tokens, int seq);
+    struct CachedStep;
+    bool ensureBuffers(int64_t tokens, int seq, const CachedStep* step = nullptr);
+    // One step over a key/value cache (Session): how many of each sequence's S
+    // rows are tokens, where they stand, and which rows' logits are wanted.
+    struct CachedStep {
+        const gbx_kv_cache* cache;
+        const int32_t* table;      // device arrays, from here
+        int maxPages;
+        const int32_t* kvLen;
+        const int32_t* nNew;
+        const int32_t* posIds;
+        float* workspace;          // of gbx_attn_cached
+        int64_t workspaceFloats;
+        std::vector<int> counts;   // host copy of nNew
+        bool even;                 // every sequence has S tokens
+        bool fresh;                // and starts here
+        bool allRows;              // logits of every row, else of each sequence's last
+    };
     // logits stay on the device; hidden_host (optional) receives forwardHidden's blocks
-    bool runForward(const std::vector<int>& tokenIDs, int batch, float* hidden_host = nullptr);
+    bool runForward(const std::vector<int>& tokenIDs, int batch, float* hidden_host = nullptr,
+                    const CachedStep* step = nullptr);
+    friend class Session;
+    bool streamAndDevice(gbx_stream_t* stream, int* device) const;   // false before loadModel
+    const float* deviceLogits() const;
+};
+
+// New: who owns which page of a paged key/value cache (host bookkeeping only, no
+// GPU).  Sequences are lists of pages and a length; forks share pages, and a
+// shared page that would be written to is replaced by a copy first.
+class PageTable {
+public:
+    struct Copies {
+        std::vector<int32_t> src, dst;   // page dst[i] is to become page src[i]
+    };
+    PageTable(int64_t pages, int pageSize);
+    int newSequence();                           // an id; ids of released sequences are used again
+    int fork(int seq);                           // an id, or -1 for an unknown sequence
+    bool release(int seq);                       // its pages, where no other sequence has them, are free again
+    bool truncate(int seq, int64_t length);      // keeps the first `length` tokens
+    // Room for n more tokens of each listed sequence (no sequence twice): pages
+    // for them, and a copy of the last page where it is shared and not full.
+    // False, with nothing changed, when the free pages do not suffice.
+    bool append(const std::vector<int>& seqs, const std::vector<int>& n, Copies* copies);
+    // Moves pages so that the pages in use are the lowest.  The targets are free
+    // pages: no target is also a source.
+    Copies compact();
+    bool known(int seq) const { return seq >= 0 && seq < (int)seqs_.size() && seqs_[seq].live; }
+    int64_t length(int seq) const { return known(seq) ? seqs_[seq].length : -1; }
+    const std::vector<int32_t>& pagesOf(int seq) const { return seqs_[seq].pages; }
+    int64_t freePages() const { return (int64_t)free_.size(); }
+    int64_t pages() const { return (int64_t)refs_.size(); }
+    int pageSize() const { return pageSize_; }
+    int references(int64_t page) const { return refs_[page]; }
+
+private:
+    struct Seq {
+        std::vector<int32_t> pages;
+        int64_t length = 0;
+        bool live = false;
+    };
+    int32_t take();
+    void drop(int32_t page);
+    int pageSize_;
+    std::vector<int> refs_;
+    std::vector<int32_t> free_;   // a heap, the lowest page first
+    std::vector<Seq> seqs_;
+};
+
+// New: cached generation.  A Session holds a paged 8-bit key/value cache of all
+// the model's layers (gbx_kv_cache) and any number of sequences in it; a step
+// costs the new tokens only, where TransformerModel::forward runs the whole
+// prefix.  Keys and values are held in 8 bits (see gbx_kv_append), so logits
+// differ from forward's by that rounding; a prompt that starts its sequences
+// attends over its unrounded keys and values.  The model must outlive the
+// session; a session is used by one thread at a time, as the model is.
+class Session {
+public:
+    Session(TransformerModel& model, int64_t pages, int pageSize = 64);
+    ~Session();
+    Session(const Session&) = delete;
+    Session& operator=(const Session&) = delete;
+
+    bool ok() const { return ok_; }
+    int newSequence() { return table_.newSequence(); }
+    // A sequence that continues from where `seq` stands; shares its pages.
+    int fork(int seq) { return table_.fork(seq); }
+    bool truncate(int seq, int64_t length) { return table_.truncate(seq, length); }
+    bool release(int seq) { return table_.release(seq); }
+    // Pages in use moved to the lowest places; how many moved, -1 on failure.
+    int64_t compact();
+    int64_t length(int seq) const { return table_.length(seq); }
+    int64_t freePages() const { return table_.freePages(); }
+
+    // Appends counts[i] tokens to sequence seqs[i] (ids: all of them, one
+    // sequence after another) and returns logits: each sequence's last token's,
+    // or with allRows every token's, vocab floats each, in the order of ids.
+    // Empty on failure (lastError()), with every sequence at the length it had.
+    std::vector<float> forward(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts,
+                               bool allRows = false);
+    // forward, and each sequence's next token by the reference's rule
+    // (gbx_select_tokens) with the draws u (one each; not used at temperature <=
+    // 0.01).  Empty on failure.
+    std::vector<int> nextTokens(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts,
+                                double temperature, const std::vector<double>& u);
+    // Speculative step: sequence i is given nDraft + 1 ids, its pending token
+    // and nDraft drafts (draftLen[i] of them count; empty: all), all are scored
+    // in one forward and the drafts verified (gbx_verify_tokens; draftLogits:
+    // [seq][nDraft][vocab], may be null; u: nDraft + 1 draws each).  outIds
+    // receives nDraft + 1 entries a sequence: the accepted drafts, the next
+    // token, -1s; accepted the counts.  Each sequence keeps its pending token and
+    // its accepted drafts; the next token is the next pending one.
+    bool verify(const std::vector<int>& seqs, const std::vector<int>& ids, int nDraft, const std::vector<int>& draftLen,
+                const float* draftLogits, double temperature, const std::vector<double>& u, std::vector<int>* outIds,
+                std::vector<int>* accepted);
+    const std::string& lastError() const { return err_; }
+
+private:
+    struct Impl;
+    bool fail(const std::string& msg);
+    bool step(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, bool allRows,
+              const std::vector<int>& padded, int S);
+    bool check(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, int* S,
+               std::vector<int>* padded);
+    TransformerModel& model_;
+    PageTable table_;
+    std::unique_ptr<Impl> impl_;
+    bool ok_ = false;
+    std::string err_;
 };
 
 // Row sharding across GPUs with one host thread per device: a replica of
