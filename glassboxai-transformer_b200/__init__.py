@@ -295,24 +295,24 @@ class _KVCacheStruct(ctypes.Structure):
 
 
 class _Torch:
-    """The three things of torch that a cache call needs, looked up once."""
-    int32 = device = stream = None
+    """The few things of torch that a cache call needs, looked up once."""
+    int32 = float32 = float64 = device = stream = None
 
     @classmethod
     def load(cls):
         import torch
-        cls.int32 = torch.int32
+        cls.int32, cls.float32, cls.float64 = torch.int32, torch.float32, torch.float64
         cls.device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else lambda: -1
         cls.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _device_of(t):
-    """CUDA device index of a tensor, or -1 (an address, a host tensor)."""
+    """CUDA device index of a tensor; -1 for an address, -2 for a host tensor."""
     if _Torch.int32 is None:
         _Torch.load()
     d = getattr(t, "device", None)
     if d is None or d.type != "cuda":
-        return -1
+        return -1 if d is None else -2
     return _Torch.device() if d.index is None else d.index
 
 
@@ -323,6 +323,8 @@ def _elsewhere(dev):
 
 def _stream_on(dev, stream):
     """Handle of the stream to launch on: `stream`, or the device's current torch stream."""
+    if dev == -2:
+        raise ValueError("the tensors are not on a GPU")
     if stream is None:
         return _Torch.stream(dev) if dev >= 0 else _stream(None)
     return stream if isinstance(stream, int) else stream.cuda_stream
@@ -377,6 +379,15 @@ def _index(name, t):
     return t.data_ptr()
 
 
+def _floats(name, t, dtype=None):
+    """Address of an array of floats: an fp32 (or `dtype`) tensor, an address or None.  It may be a strided view."""
+    if t is None or isinstance(t, int):
+        return t
+    if t.dtype is not (dtype or _Torch.float32):
+        raise ValueError(f"{name} must be a {dtype or _Torch.float32} tensor")
+    return t.data_ptr()
+
+
 def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_new=None, k_lo=None, v_lo=None,
               err_flag=None, stream=None):
     """Appends row (b, i), i < n_new[b], of k and v (row stride ld) as token
@@ -387,7 +398,8 @@ def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_
         return _there(dev, kv_append, cache, layer, k, v, table, kv_len, B=B, S=S, ld=ld, max_pages=max_pages, n_new=n_new,
                       k_lo=k_lo, v_lo=v_lo, err_flag=err_flag, stream=stream)
     rc = _lib.gbx_kv_append(cache._ref, layer, _index("table", table), table.shape[-1] if max_pages is None else max_pages,
-                            _index("kv_len", kv_len), _index("n_new", n_new), B, S, _p(k), _p(k_lo), _p(v), _p(v_lo), ld,
+                            _index("kv_len", kv_len), _index("n_new", n_new), B, S, _floats("k", k), _floats("k_lo", k_lo),
+                            _floats("v", v), _floats("v_lo", v_lo), ld,
                             _p(err_flag), _stream_on(dev, stream))
     if rc:
         _check(rc)
@@ -400,7 +412,8 @@ def kv_read(cache, layer, table, kv_len, k_out, v_out, *, B, S, ld, max_pages=No
         return _there(dev, kv_read, cache, layer, table, kv_len, k_out, v_out, B=B, S=S, ld=ld, max_pages=max_pages, n=n,
                       err_flag=err_flag, stream=stream)
     rc = _lib.gbx_kv_read(cache._ref, layer, _index("table", table), table.shape[-1] if max_pages is None else max_pages,
-                          _index("kv_len", kv_len), _index("n", n), B, S, _p(k_out), _p(v_out), ld, _p(err_flag),
+                          _index("kv_len", kv_len), _index("n", n), B, S, _floats("k_out", k_out),
+                          _floats("v_out", v_out), ld, _p(err_flag),
                           _stream_on(dev, stream))
     if rc:
         _check(rc)
@@ -436,9 +449,10 @@ def attn_cached(cache, layer, q, out, table, kv_len, *, B, S, H, ld, ld_out, sca
                       workspace_floats=workspace_floats, err_flag=err_flag, stream=stream)
     if workspace_floats is None:
         workspace_floats = workspace.numel() if hasattr(workspace, "numel") else 0
-    rc = _lib.gbx_attn_cached(cache._ref, layer, _p(q), _p(q_lo), ld, _index("table", table),
+    rc = _lib.gbx_attn_cached(cache._ref, layer, _floats("q", q), _floats("q_lo", q_lo), ld, _index("table", table),
                               table.shape[-1] if max_pages is None else max_pages, _index("kv_len", kv_len),
-                              _index("n_new", n_new), B, S, H, scale, _p(out), _p(out_lo), ld_out, _p(workspace),
+                              _index("n_new", n_new), B, S, H, scale, _floats("out", out), _floats("out_lo", out_lo),
+                              ld_out, _floats("workspace", workspace),
                               workspace_floats, _p(err_flag), _stream_on(dev, stream))
     if rc:
         _check(rc)
@@ -452,8 +466,8 @@ def verify_tokens(logits, draft_ids, out_ids, n_accepted, *, B, n_draft, vocab, 
         return _there(dev, verify_tokens, logits, draft_ids, out_ids, n_accepted, B=B, n_draft=n_draft, vocab=vocab,
                       temperature=temperature, uniforms=uniforms, draft_logits=draft_logits, draft_len=draft_len,
                       err_flag=err_flag, stream=stream)
-    rc = _lib.gbx_verify_tokens(_p(logits), _p(draft_logits), _index("draft_ids", draft_ids), _index("draft_len", draft_len), B,
-                                n_draft, vocab, temperature, _p(uniforms), _index("out_ids", out_ids),
+    rc = _lib.gbx_verify_tokens(_floats("logits", logits), _floats("draft_logits", draft_logits), _index("draft_ids", draft_ids), _index("draft_len", draft_len), B,
+                                n_draft, vocab, temperature, _floats("uniforms", uniforms, _Torch.float64), _index("out_ids", out_ids),
                                 _index("n_accepted", n_accepted), _p(err_flag), _stream_on(dev, stream))
     if rc:
         _check(rc)

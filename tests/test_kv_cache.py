@@ -106,6 +106,7 @@ def test_wrong_tensors_are_refused(gbx):
     s = torch.zeros((1, 2, 2))
     cache = gbx.KVCache(k=k, v=v, k_scale=s, v_scale=s.clone())
     assert (cache.pages, cache.heads, cache.page, cache.hd) == (2, 2, 16, 64)
+    t32 = torch.zeros((1, 2), dtype=torch.int32)
     for bad in (dict(v=v[:, :1]), dict(k_scale=s.double()), dict(v=v.float()), dict(k_scale=s[:, :1])):
         with pytest.raises(ValueError):
             gbx.KVCache(**dict(dict(k=k, v=v, k_scale=s, v_scale=s), **bad))
@@ -113,6 +114,15 @@ def test_wrong_tensors_are_refused(gbx):
         gbx.KVCache(layers=1, pages=1, heads=1, page=24, hd=64, device="cpu")
     with pytest.raises(ValueError, match="int32"):
         gbx.kv_append(cache, 0, k, k, torch.zeros((1, 2), dtype=torch.int64), 16, B=1, S=1, ld=128)
+    with pytest.raises(ValueError, match="float32"):
+        gbx.kv_append(cache, 0, s.double(), s, t32, 16, B=1, S=1, ld=128)
+    with pytest.raises(ValueError, match="float64"):
+        gbx.verify_tokens(1 << 20, None, 16, 16, B=1, n_draft=0, vocab=4, temperature=1.0, uniforms=s)
+    for call in (lambda: gbx.kv_append(cache, 0, s, s, t32, t32, B=1, S=1, ld=128),
+                 lambda: gbx.kv_copy_pages(cache, t32, t32, n=2),
+                 lambda: gbx.verify_tokens(s, None, t32, t32, B=1, n_draft=0, vocab=2)):
+        with pytest.raises(ValueError, match="not on a GPU"):
+            call()
     with pytest.raises(ValueError, match="int32"):
         gbx.kv_copy_pages(cache, torch.zeros(4, dtype=torch.int32)[::2], 16, n=2)
 

@@ -409,6 +409,62 @@ def near_table(s, near):
     return rng.permutation(m + 3)[:m].reshape(1, m)
 
 
+@pytest.mark.parametrize("P,heads,G,hd,S,before", [(16, 1, 1, 64, 20, [5000]), (64, 1, 8, 128, 3, [3000]), (32, 1, 1, 96, 66, [2500]),
+                                                   (128, 1, 2, 16, 40, [1500, 0])])
+def test_attention_of_many_rows_cut_into_pieces(gbx, cuda, P, heads, G, hd, S, before):
+    """More rows than 16 over caches long enough for several clusters, which meet in the workspace."""
+    B, H = len(before), heads * G
+    s = Setup(gbx, P, heads, hd, B, max(before) + S, seed=S)
+    q = (s.rng.standard_normal((B, S, H, hd)) * 2).astype(np.float32)
+    n_new = np.full(B, S)
+    kv_len = np.array(before) + n_new
+    assert gbx.attn_cached_workspace(s.cache, B=B, S=S, H=H, max_pages=s.m) > 0
+    want, tol = kv_oracle.attend(s.ref, s.table, kv_len, n_new, q, 9.0)
+    for ws in ("auto", None):
+        out, _ = run_attn(s, q, kv_len, n_new, 9.0, workspace=ws)
+        assert_attn(out, want, tol, np.ones(q.shape, bool))
+    assert int(s.err.item()) == 0
+
+
+@pytest.mark.parametrize("S,tokens_", [(1, 300), (1, 40000), (30, 300)])
+def test_attention_reports_a_timeout(gbx, cuda, S, tokens_):
+    """The first wait for a copy gives up at once: NaN rows and the status, and the next call is as ever."""
+    s = Setup(gbx, 16, 1, 64, 1, tokens_, seed=S)
+    q = s.rng.standard_normal((1, S, 1, 64)).astype(np.float32)
+    clean, _ = run_attn(s, q, [tokens_], [S], 8.0)
+    prev = gbx.set_first_wait_limit(0)
+    try:
+        out, _ = run_attn(s, q, [tokens_], [S], 8.0, fill=1.0)
+    finally:
+        gbx.set_first_wait_limit(prev)
+    assert np.isnan(out).all() and int(s.err.item()) == gbx.LINEAR_TIMEOUT
+    s.err.zero_()
+    again, _ = run_attn(s, q, [tokens_], [S], 8.0)
+    assert np.array_equal(clean, again) and int(s.err.item()) == 0
+
+
+def test_calls_on_two_streams(gbx, cuda):
+    """Two caches, each with its own workspace, on two streams at once."""
+    import torch
+    sets = [Setup(gbx, 16, 2, 64, 2, 3000, seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    qs = [s.rng.standard_normal((2, 1, 2, 64)).astype(np.float32) for s in sets]
+    want = [run_attn(s, q, [3000, 1700], [1, 1], 8.0)[0] for s, q in zip(sets, qs)]
+    args = []
+    for s, q in zip(sets, qs):
+        n = gbx.attn_cached_workspace(s.cache, B=2, S=1, H=2, max_pages=s.m)
+        args.append((dev(q.reshape(2, -1)), torch.empty(2, 128, device="cuda"), i32(s.table), i32([3000, 1700]), i32([1, 1]),
+                     torch.empty(max(n, 1), device="cuda")))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, st, (q, out, table, kv_len, n_new, ws) in zip(sets, streams, args):
+            gbx.attn_cached(s.cache, 0, q, out, table, kv_len, B=2, S=1, H=2, ld=128, ld_out=128, scale=8.0, n_new=n_new, workspace=ws,
+                            stream=st)
+    torch.cuda.synchronize()
+    for w, a in zip(want, args):
+        assert np.array_equal(w.reshape(2, 128), a[1].cpu().numpy())
+
+
 # ------------------------------------------------------------------ page copies
 @pytest.mark.parametrize("P,heads,hd,layers,n", [(16, 12, 64, 3, 5), (128, 1, 16, 1, 1), (32, 25, 64, 2, 40), (64, 3, 112, 4, 9)])
 def test_copy_pages(gbx, cuda, P, heads, hd, layers, n):

@@ -53,6 +53,18 @@ def test_verification_matches_the_oracle(gbx, cuda, B, n, V, T):
     assert int(err.item()) == 0
 
 
+@pytest.mark.parametrize("B,n,V,T", [(20, 2, 50257, 0.8), (40, 1, 50257, 1.0), (2, 2, 70001, 0.9), (45, 2, 140001, 0.0), (38, 1, 9000, 1.2)])
+def test_vocabularies_of_several_chunks_a_warp(gbx, cuda, B, n, V, T):
+    """Clusters of 16, 8 and 4 CTAs, whose warps go through their run in pieces."""
+    rng = np.random.default_rng(V + B)
+    logits, draft, ids, u = inputs(rng, B, n, V, T)
+    lens = rng.integers(0, n + 1, B)
+    for d in (draft, None):
+        want, wacc = kv_oracle.verify(logits, d, ids, lens, T, u)
+        got, acc = run(gbx, logits, d, ids, lens, T, u)
+        assert np.array_equal(acc, wacc) and np.array_equal(got, want)
+
+
 def test_greedy_takes_the_first_of_equal_maxima_and_needs_no_draws(gbx, cuda):
     V = 50257
     logits = np.zeros((2, 3, V), np.float32)
