@@ -3,19 +3,19 @@
 // select.cu.  No counterpart in the reference (its generate loop takes one
 // token per forward, transformer.cu:986-1036).
 //
-// One cluster of 4 to 16 CTAs per sequence, one launch; each of its warps owns
+// One cluster of 16 or 8 CTAs per sequence, one launch; each of its warps owns
 // one run of the vocabulary.
-//   A  the rows' statistics: the warp's run of every target and draft row,
-//      through a ring of four asynchronous copies; maximum and sum of
-//      2^((x - m) log2(e) / T) in one pass (running maximum per lane).  fp32:
-//      the sum decides a test whose border is a single point.
+//   A  the rows' statistics: the warp's share of every target and draft row;
+//      maximum and sum of 2^((x - m) log2(e) / T) in one pass (running maximum
+//      per lane).  fp32: the sum decides a test whose border is a single point.
 //   B  every CTA takes the same decision from the statistics and the drafted
 //      tokens' own logits: the first draft that is not accepted.
 //   C  the next token by inversion of the running sum of r_j = max(p_j - q_j,
 //      0) (p_j after the last draft): the two normalisers, the runs' sums, and
-//      then the one run that holds the border.  A lane owns 16 neighbouring
-//      entries, so a run's sum, its lanes' prefixes and the entry are found
-//      from the same 16 registers.  fp64: a vocabulary has a border every few
+//      then the one run that holds the border.  A lane owns neighbouring
+//      entries of its warp's run, whose exponentials stay in shared memory, so
+//      a run's sum, its lanes' prefixes and the entry come from one evaluation.
+//      fp64: a vocabulary has a border every few
 //      1e-5 of the sum, so an error of 1e-7 in the running sum would pick a
 //      neighbour every few hundred draws.
 // What the CTAs tell one another they write into each other's shared memory
@@ -35,16 +35,18 @@
 
 namespace gbx {
 
-constexpr int kVfWarps = 8;
-constexpr int kVfThreads = 32 * kVfWarps;
-constexpr int kVfChunk = 512;    // entries a warp handles at a time
-constexpr int kVfSlots = 4;      // chunks in flight
-constexpr int kVfPad = kVfChunk + kVfChunk / 16;   // a chunk with one float of padding after every 16
 constexpr int kVfMaxDraft = 256;
-// dynamic shared memory: the ring (later the padded chunks), then the rows' statistics
-constexpr size_t kVfRing = sizeof(float) * kVfWarps * kVfSlots * kVfChunk;
-constexpr size_t vf_smem(int n, int cluster) { return kVfRing + sizeof(float2) * (2 * n + 1) * (kVfWarps + cluster + 1); }
-static_assert(2 * kVfPad <= kVfSlots * kVfChunk, "two padded chunks fit a warp's ring");
+constexpr int kVfQuads = 2;      // 16-byte loads of a lane in one unit of A
+constexpr int kVfAhead = 2;      // units in flight
+
+// A warp's run of the vocabulary, and a lane's neighbouring entries of it (odd:
+// the lanes' doubles then lie in different banks).
+__host__ __device__ constexpr int vf_run(int vocab, int runs) { return (vocab + runs - 1) / runs; }
+__host__ __device__ constexpr int vf_seg(int run) { return ((run + 31) / 32) | 1; }
+// Dynamic shared memory: the rows' statistics, then where they fit (KEEP) the
+// exponentials of each warp's run in both distributions.
+constexpr size_t vf_stats(int n, int cluster, int warps) { return sizeof(float2) * (2 * n + 1) * (warps + cluster + 1); }
+constexpr size_t vf_kept(int vocab, int cluster, int warps) { return sizeof(double) * 2 * warps * 32 * vf_seg(vf_run(vocab, cluster * warps)); }
 
 struct VfArgs {
     const float* logits;
@@ -142,13 +144,14 @@ struct VfExp {
 };
 
 // C: CTAs of a cluster.
-template <int C>
-__global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
+// W: warps of a CTA.  KEEP: part C holds the exponentials it sums in shared memory.
+template <int C, int W, bool KEEP>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const VfArgs a)
 {
-    constexpr int kVfRuns = C * kVfWarps;
+    constexpr int kVfRuns = C * W, kVfThreads = 32 * W;
     grid_dependency_wait();
     vf_arrive();   // awaited before the first write into another CTA
-    extern __shared__ __align__(16) float vf_smem_raw[];
+    extern __shared__ __align__(16) float2 s_warp[];                                            // [rows][warps]
     __shared__ double s_root[128];
     __shared__ double s_z[2][kVfRuns], s_run[kVfRuns];
     __shared__ int s_dec;         // accepted drafts
@@ -157,45 +160,59 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
     const int64_t b = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = a.n, V = a.vocab, max_rows = 2 * n + 1;
-    float* ring = vf_smem_raw + warp * kVfSlots * kVfChunk;
-    float2* s_warp = reinterpret_cast<float2*>(vf_smem_raw + kVfWarps * kVfSlots * kVfChunk);   // [rows][warps]
-    float2* s_part = s_warp + max_rows * kVfWarps;                                              // [rows][CTAs]
-    float2* s_stat = s_part + max_rows * C;                                            // [rows]
+    float2* s_part = s_warp + max_rows * W;                                              // [rows][CTAs]
+    float2* s_stat = s_part + max_rows * C;                                                     // [rows]
     int len = a.draft_len ? a.draft_len[b] : n;
     const bool bad_len = len < 0 || len > n;
     if (bad_len) len = 0;
     const float* tl = a.logits + b * (n + 1) * (int64_t)V;
     const float* dl = a.draft_logits && !a.greedy ? a.draft_logits + b * (int64_t)n * V : nullptr;
     const int32_t* ids = a.draft_ids + b * n;
-    // this warp's run of every row, in chunks
-    const int run = (V + kVfRuns - 1) / kVfRuns;
-    const int me = (int)rank * kVfWarps + warp;
+    // this warp's run of a row in C
+    const int run = vf_run(V, kVfRuns), seg = vf_seg(run);
+    const int me = (int)rank * W + warp;
     const int j0 = min(V, me * run), j1 = min(V, j0 + run);
-    const int chunks = (run + kVfChunk - 1) / kVfChunk;
     const int nrows = bad_len ? 0 : len + 1 + (dl ? len : 0);
     auto row = [&](int k) { return k <= len ? tl + (int64_t)k * V : dl + (int64_t)(k - len - 1) * V; };
 
     // ---------------------------------------------------- A
-    // unit u: chunk u % chunks of row u / chunks
-    auto fetch = [&](int k, int ch, int slot) {
-        const float* x = row(k);
-        const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + slot * kVfChunk + lane);
-        const int j = j0 + ch * kVfChunk + lane;
-#pragma unroll
-        for (int e = 0; e < kVfChunk / 32; ++e)
-            if (j + 32 * e < j1) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 128 * e), "l"(x + j + 32 * e) : "memory");
+    // Here a warp's share of a row is a run of 16-byte quads, which start at the
+    // row's own first aligned entry; the up to six entries around them are warp
+    // 0's.  Unit u: pass u % passes (64 quads) of row u / passes, the next two
+    // units' loads in flight while one is worked on.
+    constexpr int N = kVfQuads, Q = 32 * N;
+    const int share = ((V >> 2) + kVfRuns) / kVfRuns, passes = (share + Q - 1) / Q;
+    struct Unit {
+        float4 v[N];
+        float x;    // one of the entries around the quads, or -inf
+        int j;      // v[i] holds entries j + 128 i ..
+        int jx;
     };
-    int fk = 0, fc = 0;   // the unit that is fetched next
-    auto fetch_next = [&](int slot) {
-        if (fk < nrows) fetch(fk, fc, slot);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (++fc == chunks) {
-            fc = 0;
+    auto fetch = [&](int k, int pass) {
+        const float* x = row(k);
+        const int head = min(V, (int)((4 - ((reinterpret_cast<uintptr_t>(x) >> 2) & 3)) & 3)), quads = (V - head) >> 2;
+        const int q0 = me * share + pass * Q + lane, q1 = min(quads, (me + 1) * share);
+        Unit u;
+        u.j = head + 4 * q0;
+        const float4* at = reinterpret_cast<const float4*>(x + head) + q0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) u.v[i] = q0 + 32 * i < q1 ? at[32 * i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        const int tail = V - head - 4 * quads;
+        u.jx = lane < 4 ? lane : head + 4 * quads + lane - 4;
+        u.x = me == 0 && pass == 0 && (lane < 4 ? lane < head : lane - 4 < tail) ? x[u.jx] : -INFINITY;
+        return u;
+    };
+    int fk = 0, fp = 0;   // the unit that is fetched next
+    Unit next[kVfAhead];
+    auto fetch_next = [&](Unit& u) {
+        if (fk < nrows) u = fetch(fk, fp);
+        if (++fp == passes) {
+            fp = 0;
             ++fk;
         }
     };
 #pragma unroll
-    for (int i = 0; i < kVfSlots - 1; ++i) fetch_next(i);
+    for (int i = 0; i < kVfAhead; ++i) fetch_next(next[i]);
     // what B and C need from memory, asked for meanwhile
     const double u_next = a.greedy ? 0.0 : a.uniforms[b * (n + 1) + n];
     int d_mine = -1;
@@ -211,45 +228,41 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
     }
     if (tid < 128) s_root[tid] = exp2(tid * (1.0 / 128.0));
     if (tid == 0) s_dec = len;
-    int slot = 0;
-#pragma unroll 2
     for (int k = 0; k < nrows; ++k) {
         float m = -INFINITY, s = 0.0f;
         int at = 0x7fffffff;
         bool nan = false;
-        for (int ch = 0; ch < chunks; ++ch) {
-            __syncwarp();   // every lane has read the slot that is filled next
-            fetch_next(slot ? slot - 1 : kVfSlots - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kVfSlots - 1) : "memory");
-            __syncwarp();
-            float v[kVfChunk / 32];
-            const int j = j0 + ch * kVfChunk + lane;
-#pragma unroll
-            for (int e = 0; e < kVfChunk / 32; ++e) v[e] = j + 32 * e < j1 ? ring[slot * kVfChunk + lane + 32 * e] : -INFINITY;
+        for (int pass = 0; pass < passes; ++pass) {
+            const Unit u = next[0];
+            next[0] = next[1];
+            fetch_next(next[1]);
+            static_assert(N == 2 && kVfAhead == 2, "as written out here");
+            const float v[4 * N + 1] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w, u.v[1].x, u.v[1].y, u.v[1].z, u.v[1].w, u.x};
             if (a.greedy) {
 #pragma unroll
-                for (int e = 0; e < kVfChunk / 32; ++e) {
+                for (int e = 0; e <= 4 * N; ++e) {
+                    const int j = e == 4 * N ? u.jx : u.j + 128 * (e >> 2) + (e & 3);
                     nan |= v[e] != v[e];
-                    if (v[e] > m) {
+                    if (v[e] > m || (v[e] == m && j < at)) {
                         m = v[e];
-                        at = j + 32 * e;
+                        at = j;
                     }
                 }
             } else {
-                float bm = fmaxf(m, v[0]);
+                float bm = fmaxf(m, v[4 * N]);
 #pragma unroll
-                for (int e = 1; e < kVfChunk / 32; ++e) bm = fmaxf(bm, v[e]);
+                for (int e = 0; e < 4 * N; ++e) bm = fmaxf(bm, v[e]);
                 const float base = (bm == -INFINITY ? 0.0f : bm) * a.c2;
-                float t = 0.0f, t1 = 0.0f;
+                const float2 by = splat2(a.c2), less = splat2(-base);
+                float2 t = make_float2(vf_exp2(fmaf(v[4 * N], a.c2, -base)), 0.0f);   // a NaN makes the sum NaN
 #pragma unroll
-                for (int e = 0; e < kVfChunk / 32; e += 2) {   // a NaN makes the sum NaN
-                    t += vf_exp2(fmaf(v[e], a.c2, -base));
-                    t1 += vf_exp2(fmaf(v[e + 1], a.c2, -base));
+                for (int e = 0; e < 4 * N; e += 2) {
+                    const float2 y = __ffma2_rn(make_float2(v[e], v[e + 1]), by, less);
+                    t = __fadd2_rn(t, make_float2(vf_exp2(y.x), vf_exp2(y.y)));
                 }
-                s = fmaf(s, vf_exp2(fmaf(m, a.c2, -base)), t + t1);   // m = -inf: 0
+                s = fmaf(s, vf_exp2(fmaf(m, a.c2, -base)), t.x + t.y);             // m = -inf: 0
                 m = bm;
             }
-            slot = slot + 1 == kVfSlots ? 0 : slot + 1;
         }
         float2 st;
         if (a.greedy) {
@@ -258,17 +271,16 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
             const float wm = group_max<32>(m), base = wm == -INFINITY ? 0.0f : wm;
             st = make_float2(wm, group_sum<32>(s * vf_exp2((m - base) * a.c2)));
         }
-        if (lane == 0) s_warp[k * kVfWarps + warp] = st;
+        if (lane == 0) s_warp[k * W + warp] = st;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     vf_wait();   // the other CTAs run
     // this CTA's part of each row, to every CTA
-    for (int i = tid; i < (nrows * kVfWarps + 31 & ~31); i += kVfThreads) {
-        const int k = i / kVfWarps, w = i % kVfWarps;
-        const float2 t = vf_reduce<kVfWarps>(k < nrows ? s_warp[i] : make_float2(-INFINITY, 0.0f), a.c2, a.greedy);
+    for (int i = tid; i < (nrows * W + 31 & ~31); i += kVfThreads) {
+        const int k = i / W, w = i % W;
+        const float2 t = vf_reduce<W>(k < nrows ? s_warp[i] : make_float2(-INFINITY, 0.0f), a.c2, a.greedy);
         if (k < nrows)
-            for (uint32_t p = w; p < C; p += kVfWarps) vf_push(s_part + k * C + rank, p, t);
+            for (uint32_t p = w; p < C; p += W) vf_push(s_part + k * C + rank, p, t);
     }
     vf_arrive();
     vf_wait();
@@ -329,44 +341,37 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
     const float* qx = rejected && dl ? dl + (int64_t)acc * V : nullptr;
     const int hot = rejected && !dl ? ids[acc] : -1;   // a draft picked without chance
     const VfExp pexp(sp.x, a.inv_t, s_root), qexp(sq.x, a.inv_t, s_root);
-    // e^((x - m) / T) of entries j0 + 512 ch + 16 lane + e: read coalesced, turned in shared memory
-    double ep[16], eq[16];
-    auto load = [&](int ch) {
-        const int j = j0 + ch * kVfChunk + lane;
-        float x[16], y[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = j + 32 * e < j1 ? px[j + 32 * e] : -INFINITY;
-        if (qx)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = j + 32 * e < j1 ? qx[j + 32 * e] : -INFINITY;
-        __syncwarp();
-        float* turn = ring + lane + (lane >> 4);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            turn[34 * e] = x[e];
-            if (qx) turn[kVfPad + 34 * e] = y[e];
-        }
-        __syncwarp();
-        const float* mine = ring + 17 * lane;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) ep[e] = pexp(mine[e]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) eq[e] = qx ? qexp(mine[kVfPad + e]) : 0.0;
-    };
+    // the run's e^((x - m) / T), kept or formed again; entry i of this lane's is i of the run
+    double* kept_p = reinterpret_cast<double*>(s_stat + max_rows + (max_rows & 1)) + warp * 2 * 32 * seg;
+    double* kept_q = kept_p + 32 * seg;
+    auto prob = [&](int i) { return KEEP ? kept_p[i] : j0 + i < j1 ? pexp(px[j0 + i]) : 0.0; };
+    auto other = [&](int i) { return !qx ? 0.0 : KEEP ? kept_q[i] : j0 + i < j1 ? qexp(qx[j0 + i]) : 0.0; };
     auto sum32 = [](double v) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     };
     double zp = 0.0, zq = 0.0;
-    for (int ch = 0; ch < chunks; ++ch) {
-        load(ch);
+    for (int i = lane; i < 32 * seg; i += 128) {   // four loads of each row before their use
+        float x[4], y[4];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            zp += ep[e];
-            zq += eq[e];
+        for (int e = 0; e < 4; ++e) {
+            const int j = j0 + i + 32 * e;
+            x[e] = j < j1 ? px[j] : -INFINITY;
+            y[e] = qx && j < j1 ? qx[j] : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double p = pexp(x[e]), q = qx ? qexp(y[e]) : 0.0;
+            zp += p;
+            zq += q;
+            if (KEEP && i + 32 * e < 32 * seg) {
+                kept_p[i + 32 * e] = p;
+                kept_q[i + 32 * e] = q;
+            }
         }
     }
+    __syncwarp();
     zp = sum32(zp);
     zq = sum32(zq);
     if (lane < C) {
@@ -384,12 +389,11 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
     }
     const double ip = 1.0 / sum32(zp), iq = qx ? 1.0 / sum32(zq) : 0.0;
     bool minus = rejected;
-    // entry e's weight of the chunk that is loaded
-    auto weight = [&](int ch, int e) {
+    auto weight = [&](int i) {
         // rounded products: equal p and q leave exactly nothing, and every evaluation the same
-        const double p = __dmul_rn(ep[e], ip);
+        const double p = __dmul_rn(prob(i), ip);
         if (!minus) return p;
-        const double q = qx ? __dmul_rn(eq[e], iq) : j0 + ch * kVfChunk + 16 * lane + e == hot ? 1.0 : 0.0;
+        const double q = qx ? __dmul_rn(other(i), iq) : j0 + i == hot ? 1.0 : 0.0;
         return p > q ? __dsub_rn(p, q) : 0.0;
     };
     auto scan32 = [&](double v) {   // inclusive
@@ -401,13 +405,10 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
         return v;
     };
     for (;;) {
-        double t = 0.0;
-        for (int ch = 0; ch < chunks; ++ch) {
-            if (chunks > 1) load(ch);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) t += weight(ch, e);
-        }
-        t = sum32(t);
+        double mine_sum = 0.0;   // of this lane's entries
+#pragma unroll 4
+        for (int i = lane * seg; i < (lane + 1) * seg; ++i) mine_sum += weight(i);
+        const double mine_incl = scan32(mine_sum), t = __shfl_sync(0xffffffffu, mine_incl, 31);
         if (lane < C) vf_push(&s_run[me], lane, t);
         vf_arrive();
         vf_wait();
@@ -443,50 +444,39 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_kernel(const VfArgs a)
         // none (u * all rounded up to all): the last entry with any weight
         const int owner = who ? __ffs(who) - 1 : 31 - __clz(some);
         found = __shfl_sync(0xffffffffu, who ? found : any, owner);
-        double cum = __shfl_sync(0xffffffffu, at_run, owner);
+        const double cum = __shfl_sync(0xffffffffu, at_run, owner);
         if (found != me) return;
-        int pick = -1, last = -1;   // last: the run's last entry with any weight, should rounding end the run early
-        for (int ch = 0; ch < chunks && pick < 0; ++ch) {
-            if (chunks > 1) load(ch);
-            double w[16], sum = 0.0;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                w[e] = weight(ch, e);
-                sum += w[e];
+        // the entry, and the run's last one with any weight, should rounding end the run early
+        double at = cum + (mine_incl - mine_sum);
+        int pick = 0x7fffffff, last = -1;
+        for (int i = lane * seg; i < (lane + 1) * seg; ++i) {
+            const double w = weight(i);
+            at += w;
+            if (w > 0.0) {
+                last = j0 + i;
+                if (at > want) pick = min(pick, j0 + i);
             }
-            const double c = scan32(sum);
-            double at = cum + (c - sum);
-            int first = 0x7fffffff, tail = -1;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                at += w[e];
-                if (w[e] > 0.0) {
-                    tail = e;
-                    if (at > want) first = min(first, e);
-                }
-            }
-            const int j = j0 + ch * kVfChunk + 16 * lane;
-            first = __reduce_min_sync(0xffffffffu, first == 0x7fffffff ? first : j + first);
-            last = max(last, __reduce_max_sync(0xffffffffu, tail < 0 ? -1 : j + tail));
-            if (first != 0x7fffffff) pick = first;
-            cum += __shfl_sync(0xffffffffu, c, 31);
         }
-        if (lane == 0) a.out_ids[b * (n + 1) + acc] = pick >= 0 ? pick : last;
+        pick = __reduce_min_sync(0xffffffffu, pick);
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (lane == 0) a.out_ids[b * (n + 1) + acc] = pick != 0x7fffffff ? pick : last;
         return;
     }
 }
 
-template <int C>
-static int vf_launch(const VfArgs& a, int64_t B, cudaStream_t s)
+template <int C, int W>
+static int vf_launch(const VfArgs& a, int64_t B, const DeviceInfo& di, cudaStream_t s)
 {
-    auto k = verify_kernel<C>;
-    const size_t smem = vf_smem(a.n, C);
+    const size_t stats = vf_stats(a.n, C, W) + 8, kept = a.greedy ? 0 : vf_kept(a.vocab, C, W);
+    const bool keep = stats + kept + 8192 <= (size_t)di.max_smem_optin;
+    const size_t smem = stats + (keep ? kept : 0);
+    auto k = keep ? verify_kernel<C, W, true> : verify_kernel<C, W, false>;
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
         (C > 8 && cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
         return check_launch("gbx_verify_tokens: launch attributes");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * C));
-    cfg.blockDim = dim3(kVfThreads);
+    cfg.blockDim = dim3(32 * W);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -537,15 +527,10 @@ extern "C" int gbx_verify_tokens(const float* logits, const float* draft_logits,
     a.out_ids = out_ids;
     a.n_accepted = n_accepted;
     a.err = err_flag;
-    // CTAs per sequence: the fewer, the less is spent on meeting; 16 while every
-    // sequence's cluster then still runs at once (two CTAs to an SM), else 8, else 4
+    // One sequence of 4 drafts, 16 and 64 of up to 7, vocabulary 50257: 16, 30 and 79 us with
+    // clusters of 16 CTAs of 8 warps, 19, 41 and 68 with 8 of 16, 26, 41 and 85 with 4 of 16.
     DeviceInfo di;
     if (device_info(&di) != GBX_OK) return GBX_ECUDA;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#ifdef VFC
-    return vf_launch<VFC>(a, B, s);
-#endif
-    if (B * 16 <= 2 * di.sm_count) return vf_launch<16>(a, B, s);
-    if (B * 8 <= 2 * di.sm_count) return vf_launch<8>(a, B, s);
-    return vf_launch<4>(a, B, s);
+    return B * 16 <= 2 * di.sm_count ? vf_launch<16, 8>(a, B, di, s) : vf_launch<8, 16>(a, B, di, s);
 }

@@ -53,9 +53,10 @@ def test_verification_matches_the_oracle(gbx, cuda, B, n, V, T):
     assert int(err.item()) == 0
 
 
-@pytest.mark.parametrize("B,n,V,T", [(20, 2, 50257, 0.8), (40, 1, 50257, 1.0), (2, 2, 70001, 0.9), (45, 2, 140001, 0.0), (38, 1, 9000, 1.2)])
-def test_vocabularies_of_several_chunks_a_warp(gbx, cuda, B, n, V, T):
-    """Clusters of 16, 8 and 4 CTAs, whose warps go through their run in pieces."""
+@pytest.mark.parametrize("B,n,V,T", [(20, 2, 50257, 0.8), (40, 1, 50257, 1.0), (2, 2, 70001, 0.9), (45, 2, 140001, 0.0), (38, 1, 9000, 1.2),
+                                        (20, 1, 140001, 0.9)])
+def test_large_vocabularies(gbx, cuda, B, n, V, T):
+    """Clusters of 16 and 8 CTAs; exponentials kept in shared memory, and too many to be kept."""
     rng = np.random.default_rng(V + B)
     logits, draft, ids, u = inputs(rng, B, n, V, T)
     lens = rng.integers(0, n + 1, B)
