@@ -56,7 +56,9 @@ namespace gbx {
 constexpr int kAcTile = 64;      // tokens per warp and step
 constexpr int kAcMaxCluster = 8;
 constexpr float kAcMagicF = 12582912.0f;        // 1.5 * 2^23, bits 0x4b400000
-constexpr float kAcQTop = 8355711.0f;           // 0x7f7f7f: the largest x whose balanced digits fit in 8 bits
+// The largest x whose balanced digits fit in 8 bits is 0x7f7f7f = 8355711; a row's
+// largest entry becomes this, to a relative 2^-22.
+constexpr float kAcQTop = 8355704.0f;
 // A weight is 2^(x - max + 23 - 2^-19): just below 2^23 at most, so that adding 2^23
 // leaves it, rounded, in the low 23 bits of the float.
 constexpr float kAcPOff = 22.99999809265137f;
@@ -272,7 +274,7 @@ __device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int
         limit[rt] = ok ? u.seq.len - u.seq.n + (int)fast_div(u.r0 + r, a.by_g) + 1 : 0;
         const int64_t at = ac_row(a, u, r, a.ld);
         float x[NCH][16];
-        float big = 0.0f, bad = 0.0f;
+        uint32_t top = 0;   // the largest |x|, as bits: NaN and infinity on top
 #pragma unroll
         for (int ch = 0; ch < NCH; ++ch) {
             const int col = 64 * ch + 16 * cc;
@@ -296,15 +298,12 @@ __device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int
                 x[ch][e + 3] = v.w;
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                big = fmaxf(big, fabsf(x[ch][e]));
-                bad = fmaf(x[ch][e], 0.0f, bad);   // NaN where an entry is not finite
-            }
+            for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[ch][e]) & 0x7fffffffu);
         }
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        bad += __shfl_xor_sync(0xffffffffu, bad, 1);
-        bad += __shfl_xor_sync(0xffffffffu, bad, 2);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float bad = top >= 0x7f800000u ? __int_as_float(0x7fc00000) : 0.0f;
+        float big = __uint_as_float(top);
         // tiny rows are first brought up exactly, so that kAcQTop / big stays finite
         const float lift = big < 8.67361738e-19f ? 1.20892582e24f : 1.0f;   // 2^-60, 2^80
         big *= lift;
@@ -317,7 +316,8 @@ __device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int
                 uint32_t y[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float f = fminf(fmaxf(x[ch][4 * w + e] * lift * up, -kAcQTop), kAcQTop);
+                    // at most 8355711 in size but for rows that are not finite, whose digits do not count
+                    const float f = x[ch][4 * w + e] * lift * up;
                     // balanced digits: the bytes of x + 0x808080, each less 128
                     y[e] = (uint32_t)(__float2int_rn(f) + 0x808080);
                 }
@@ -615,49 +615,54 @@ struct AcMeet {
 };
 
 // Starts the copies of steps into ring slots: called by a whole warp.
+constexpr int kAcArrivals = 12;   // on a slot's barrier, each phase
+
 template <int HD>
 struct AcCopies {
     const KvLayer& c;
-    const AcUnit& u;
-    int maxlim, steps, lg16;
+    const int32_t* table;   // the sequence's row
+    int h, maxlim, lg16;
     uint32_t ring;
     float* scales;   // [4][2][4]: key and value scales of the four groups
-    __device__ __forceinline__ AcCopies(const KvLayer& c_, const AcUnit& u_, int maxlim_, int steps_, uint32_t ring_, float* scales_)
-        : c(c_), u(u_), maxlim(maxlim_), steps(steps_), lg16(c_.log_page - 4), ring(ring_), scales(scales_)
+    __device__ __forceinline__ AcCopies(const KvLayer& c_, const AcUnit& u, int maxlim_, uint32_t ring_, float* scales_)
+        : c(c_), table(c_.table + (int64_t)u.b * c_.max_pages), h(u.h), maxlim(maxlim_), lg16(c_.log_page - 4), ring(ring_), scales(scales_)
     {
     }
 
-    // The page of this lane's group (lane & 3) of a step; -1: not in the pool, -2: past the last key.
-    __device__ __forceinline__ int look(int step) const
+    // The (page, head) of this lane's group (lane & 3) of a step; -1: the page is not in the pool, -2: past the last key.
+    __device__ __forceinline__ int64_t look(int step) const
     {
         const int g = 4 * step + (threadIdx.x & 3);
-        return step < steps && 16 * g < maxlim ? kv_page(c, u.b, g >> lg16) : -2;
+        if (16 * g >= maxlim) return -2;
+        const int p = table[g >> lg16];
+        return (unsigned)p < (unsigned)c.pages ? (int64_t)p * c.heads + h : -1;
     }
 
     // The keys (which = 0) or values of a step into slot s, and with the keys
     // the groups' scales into [place], -0 standing for those of a group that
-    // cannot be read.  A slot's phase is lane 0's arrival with the byte count
-    // and one of each of lanes 0-7.
-    __device__ __forceinline__ void issue(int which, int step, int place, int s, uint32_t bar, int page) const
+    // cannot be read.  A slot's phase is twelve arrivals: lanes 0-3's, each
+    // announcing its copy's bytes, and one of each of lanes 0-7.
+    __device__ __forceinline__ void issue(int which, int step, int place, int s, uint32_t bar, int64_t ph) const
     {
-        const int lane = threadIdx.x & 31, cc = lane & 3;
-        const unsigned valid = __ballot_sync(0xffffffffu, page >= 0) & 0xfu;
-        if (lane == 0) tc::mbar_arrive_expect_tx(bar, (uint32_t)__popc(valid) * 16u * HD);
-        __syncwarp();
-        if (lane < 8) {
-            const int64_t ph = (int64_t)page * c.heads + u.h;
-            if (lane < 4 && page >= 0)
+        const int lane = threadIdx.x & 31;
+        if (lane >= 8) return;
+        if (lane < 4) {
+            if (ph >= 0) {
+                tc::mbar_arrive_expect_tx(bar, 16u * HD);
                 tc::bulk_load(ring + s * 4 * ac_pitch(HD) + lane * ac_pitch(HD),
-                              (which ? c.v : c.k) + (ph << c.log_page) * HD + ((4 * step + cc) & ((1 << lg16) - 1)) * 16 * HD, 16u * HD, bar);
-            float* to = scales + place * 8 + lane;
-            if (which == 0 && page >= 0) {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(to)), "l"((lane < 4 ? c.ks : c.vs) + ph) : "memory");
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+                              (which ? c.v : c.k) + (ph << c.log_page) * HD + ((4 * step + lane) & ((1 << lg16) - 1)) * 16 * HD, 16u * HD, bar);
             } else {
-                if (which == 0) *to = -0.0f;
                 tc::mbar_arrive(bar);
+                if (which == 0 && ph == -1) kv_flag(c.err, GBX_KV_BAD_PAGE);
             }
-            if (which == 0 && page == -1 && lane < 4) kv_flag(c.err, GBX_KV_BAD_PAGE);
+        }
+        float* to = scales + place * 8 + lane;
+        if (which == 0 && ph >= 0) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(to)), "l"((lane < 4 ? c.ks : c.vs) + ph) : "memory");
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+        } else {
+            if (which == 0) *to = -0.0f;
+            tc::mbar_arrive(bar);
         }
     }
 };
@@ -695,7 +700,7 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
     const uint32_t ring = tc::smem_u32(ac_smem) + warp * NS * slot_bytes;
     const uint32_t bar0 = tc::smem_u32(&bars[warp][0]);
     if (lane == 0) {
-        for (int s = 0; s < NS; ++s) tc::mbar_init(bar0 + 8 * s, 9);
+        for (int s = 0; s < NS; ++s) tc::mbar_init(bar0 + 8 * s, kAcArrivals);
         tc::fence_mbar_init();
     }
     if (threadIdx.x == 0) s_abort = 0;
@@ -705,14 +710,14 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
     const int steps = (maxlim + kAcTile - 1) / kAcTile;
     const int stride = (int)csize * a.nsplit * W;
     const int first = (split * (int)csize + (int)rank) * W + warp;
-    const AcCopies<HD> copies(c, u, maxlim, steps, ring, &s_scale[warp][0][0][0]);
+    const AcCopies<HD> copies(c, u, maxlim, ring, &s_scale[warp][0][0][0]);
     // of this warp's k-th step
     auto look = [&](int step) { return copies.look(step); };
-    auto issue = [&](int which, int k, int s, int page) { copies.issue(which, first + k * stride, k & 3, s, bar0 + 8 * s, page); };
+    auto issue = [&](int which, int k, int s, int64_t ph) { copies.issue(which, first + k * stride, k & 3, s, bar0 + 8 * s, ph); };
 
     // pages of steps k + 1 and k + 2 of this warp while it works on step k
     static_assert(NS == 3 || NS == 4, "the page look-ahead below is two steps");
-    int pg[3];
+    int64_t pg[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k) pg[k] = look(first + k * stride);
     int issued = 0, read = 0;   // operations
@@ -838,7 +843,7 @@ __global__ void __launch_bounds__(32 * (W + 1)) attn_cached_rows_kernel(const Ac
     auto empty = [&](int s) { return bar0 + 8 * (NS + s); };
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
-            tc::mbar_init(full(s), 9);
+            tc::mbar_init(full(s), kAcArrivals);
             tc::mbar_init(empty(s), W);
         }
         s_abort = 0;
@@ -862,14 +867,16 @@ __global__ void __launch_bounds__(32 * (W + 1)) attn_cached_rows_kernel(const Ac
     }
     if (warp == W) {
         // ------------------------------------------------ the copies
-        AcCopies<HD> copies(c, u, maxlim, steps, ring, &s_scale[0][0][0]);
-        int issued = 0, page = copies.look(first);
+        AcCopies<HD> copies(c, u, maxlim, ring, &s_scale[0][0][0]);
+        int issued = 0;
+        int64_t page = copies.look(first);
         for (int step = first; step < steps; step += stride) {
-            const int next = copies.look(step + stride);
+            const int64_t next = copies.look(step + stride);
             for (int which = 0; which < 2; ++which, ++issued) {
                 const int s = issued % NS;
                 if (issued >= NS && !tc::mbar_wait(empty(s), (issued / NS - 1) & 1, abort, kDeviceWaitNs)) goto stop;
                 copies.issue(which, step, (issued >> 1) & 3, s, full(s), page);
+                __syncwarp();
             }
             page = next;
         }

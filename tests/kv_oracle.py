@@ -79,7 +79,7 @@ def attend(cache, table, kv_len, n_new, q, scale, skip=()):
     bound on an fp32-grade kernel's error at each entry.
 
     A query enters as 24-bit fixed point: every entry is off by at most qmax 2^-23
-    (half a unit of qmax / 8355711, and the rounding of the product that scales
+    (half a unit of qmax / 8355704, and the rounding of the product that scales
     it), so with B_t = qmax sum_i |k_ti| / scale and A_t = sum_i |q_i k_ti| /
     scale the score x_t (in units of log 2) is off by B 2^-23, plus the fp32
     joining of three exact sums and its scaling by three factors (8 roundings
