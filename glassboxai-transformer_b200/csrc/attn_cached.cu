@@ -35,7 +35,11 @@
 // bulk copies (cp.async.bulk, one per group and operand, straight from the
 // pages; 16 hd bytes each) a step or two ahead of its arithmetic.  Legacy
 // mma.sync is the right form here: a tile has 1 to 8 useful rows and 64 keys
-// that are used once, where a tcgen05 tile wants 128 rows.
+// that are used once, where a tcgen05 tile wants 128 rows.  256 sequences x 25
+// heads x 2048 tokens take 254 us (6.6 TB/s, the measured copy rate) in a burst
+// and 303 under the power cap, where the lower clock brings the arithmetic (230
+// us from L2) near the copies (239 alone); 2 x 8 heads x 120,001 tokens of width
+// 128 with 4 query heads each take 90 us (5.5 TB/s).
 //
 // A cluster of CTAs shares one (sequence, key head, row block): its warps take
 // the 64-token steps in turn and meet in shared memory, the CTAs through
@@ -814,7 +818,12 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
 // Many rows (the next tokens of a prompt): a CTA's W warps take 16 rows each and
 // go through the same steps, whose copies a warp of its own keeps in flight in
 // one ring.  The int8 tensor path bounds it: 16 rows x 64 tokens of width 64 are
-// 96 instructions of 8 cycles, and half as many exponentials as those take.
+// 96 instructions of 8 cycles, and half as many exponentials as those take.  2 x
+// 512 rows x 16 heads over 2048 tokens take 59 us with 31% of the tensor cycles
+// used: two warps to a scheduler do not cover each other's dependent
+// instructions.  Measured and not kept: 2 or 8 warps to a CTA (63 and 67 us),
+// two CTAs that split the steps (79), the next step's scores formed beside this
+// one's softmax (244 registers, 82 us).
 template <int HD, int W, int NS>
 __global__ void __launch_bounds__(32 * (W + 1)) attn_cached_rows_kernel(const AcArgs a)
 {
@@ -994,7 +1003,8 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, Ac
     const int G = H / c->heads;
     const int64_t rows = (int64_t)S * G;
     // 8 or 16 rows that the warps share, splitting the steps; from 17 on 64 rows that
-    // split the warps, going through the steps together
+    // split the warps, going through the steps together (4 x 20 rows of 4 query heads
+    // to a key head of width 128 over 2000 tokens: 24 us against 32 in blocks of 16)
     p->rt = rows <= 8 ? 1 : rows <= 16 ? 2 : 8;
     const bool many = p->rt == 8;
     const int R = 8 * p->rt, W = many ? 1 : kAcWarps;   // warps that split the steps

@@ -2,7 +2,8 @@
  * gbx.h -- C ABI of the B200 (sm_100a) layer-kernel hot path for
  * GlassBoxAI-Transformer: token+position embedding gather/add from GGUF
  * f32/f16/bf16 tables, residual-add + LayerNorm, bias + GELU(tanh), and the
- * row softmax.
+ * row softmax; and cached generation: a paged 8-bit key/value cache with its
+ * attention, page copies and the verification of drafted tokens.
  *
  * Conventions (all entry points):
  *   - Every pointer argument is a DEVICE pointer unless its name ends in
@@ -78,13 +79,15 @@ int gbx_set_pdl(int enable);
 
 /*
  * Limit of the first consumer wait of the staged embedding (the CTA waiting
- * for its table rows' bulk copies) and of the tensor-core contractions (the
- * MMA thread waiting for its first tile loads), process-wide, in ns of
+ * for its table rows' bulk copies), of the tensor-core contractions (the
+ * MMA thread waiting for its first tile loads) and of gbx_attn_cached (each
+ * warp waiting for its first keys), process-wide, in ns of
  * %globaltimer time; 1 s by default, like every other device wait here.  0
  * makes that wait give up at once, so a test can drive the timeout path:
  * the kernel sets GBX_EMBED_TIMEOUT / GBX_LINEAR_TIMEOUT in *err_flag, waits
  * (with the full 1 s limit) for the copies or MMAs it already started,
- * frees what it holds and returns, leaving its outputs unwritten.  No
+ * frees what it holds and returns, leaving its outputs unwritten
+ * (gbx_attn_cached: NaN).  No
  * counterpart in the reference (whose CUDA_CHECK exits the process,
  * transformer.cu:24-32).  Returns the previous limit.  For tests only.
  */
