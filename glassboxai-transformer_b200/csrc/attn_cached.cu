@@ -996,12 +996,14 @@ struct AcPlan {
     int64_t units, ws_floats;
 };
 
-static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, AcPlan* p)
+// cut: units may be cut into pieces that meet in a workspace.
+static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bool cut, AcPlan* p)
 {
-    DeviceInfo di;
-    if (device_info(&di) != GBX_OK) return GBX_ECUDA;
     const int G = H / c->heads;
     const int64_t rows = (int64_t)S * G;
+    if (rows > (1 << 30)) return set_error(GBX_ERANGE, "gbx_attn_cached: %d rows of %d query heads a key head", S, G);
+    DeviceInfo di;
+    if (device_info(&di) != GBX_OK) return GBX_ECUDA;
     // 8 or 16 rows that the warps share, splitting the steps; from 17 on 64 rows that
     // split the warps, going through the steps together (4 x 20 rows of 4 query heads
     // to a key head of width 128 over 2000 tokens: 24 us against 32 in blocks of 16)
@@ -1026,7 +1028,7 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, Ac
     p->csize = 1;
     p->nsplit = 1;
     while (p->csize < kAcMaxCluster && 2 * p->csize <= share) p->csize *= 2;
-    if (share >= 2 * kAcMaxCluster) {
+    if (share >= 2 * kAcMaxCluster && cut) {
         int64_t best = 0;
         for (int cs = kAcMaxCluster; cs >= 1; cs /= 2) {
             const int64_t ns = share / cs > 64 ? 64 : share / cs;
@@ -1087,7 +1089,7 @@ extern "C" int64_t gbx_attn_cached_workspace(const gbx_kv_cache* cache_host, int
         return -set_error(GBX_EINVAL, "gbx_attn_cached_workspace: B=%d S=%d H=%d max_pages=%d", B, S, H, max_pages);
     if (B == 0 || S == 0) return 0;
     AcPlan p;
-    if (int rc = ac_plan(cache_host, B, S, H, max_pages, &p)) return -rc;
+    if (int rc = ac_plan(cache_host, B, S, H, max_pages, true, &p)) return -rc;
     return p.ws_floats;
 }
 
@@ -1120,8 +1122,9 @@ extern "C" int gbx_attn_cached(const gbx_kv_cache* cache_host, int layer, const 
             return set_error(GBX_EINVAL, "gbx_attn_cached: an output overlaps the queries or the other output");
     }
     AcPlan p;
-    if (int rc = ac_plan(cache_host, B, S, H, max_pages, &p)) return rc;
-    if (!workspace || workspace_floats < p.ws_floats) p.nsplit = 1;
+    if (int rc = ac_plan(cache_host, B, S, H, max_pages, workspace != nullptr, &p)) return rc;
+    if (workspace_floats < p.ws_floats)
+        if (int rc = ac_plan(cache_host, B, S, H, max_pages, false, &p)) return rc;
     a.q_hi = q_hi;
     a.q_lo = q_lo;
     a.ld = ld;

@@ -258,42 +258,47 @@ class Session:
         except Exception:
             pass
 
+    def _open(self):
+        if not self.h or not self.model.h:
+            raise _gbx.GbxError(1, "the session or its model is closed")
+        return self.h
+
     def new(self) -> int:
         """An empty sequence."""
-        seq = lib().gbx_session_new(self.h)
+        seq = lib().gbx_session_new(self._open())
         if seq < 0:
             raise _err(1)
         return seq
 
     def fork(self, seq: int) -> int:
         """A sequence that continues from where `seq` stands (its pages are shared until written to)."""
-        new = lib().gbx_session_fork(self.h, seq)
+        new = lib().gbx_session_fork(self._open(), seq)
         if new < 0:
             raise _err(1)
         return new
 
     def truncate(self, seq: int, length: int):
-        rc = lib().gbx_session_truncate(self.h, seq, length)
+        rc = lib().gbx_session_truncate(self._open(), seq, length)
         if rc:
             raise _err(rc)
 
     def release(self, seq: int):
-        rc = lib().gbx_session_release(self.h, seq)
+        rc = lib().gbx_session_release(self._open(), seq)
         if rc:
             raise _err(rc)
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest places; how many moved."""
-        n = lib().gbx_session_compact(self.h)
+        n = lib().gbx_session_compact(self._open())
         if n < 0:
             raise _err(4)
         return n
 
     def length(self, seq: int) -> int:
-        return lib().gbx_session_length(self.h, seq)
+        return lib().gbx_session_length(self._open(), seq)
 
     def free_pages(self) -> int:
-        return lib().gbx_session_free_pages(self.h)
+        return lib().gbx_session_free_pages(self._open())
 
     @staticmethod
     def _rows(seqs, tokens):
@@ -310,7 +315,7 @@ class Session:
         sequence's last token, or of every token in order."""
         seqs, ids, counts = self._rows(seqs, tokens)
         out = np.empty((ids.size if all_rows else seqs.size, self.vocab), dtype=np.float32)
-        rc = lib().gbx_session_forward(self.h, _np_ptr(seqs), seqs.size, _np_ptr(ids), ids.size, _np_ptr(counts),
+        rc = lib().gbx_session_forward(self._open(), _np_ptr(seqs), seqs.size, _np_ptr(ids), ids.size, _np_ptr(counts),
                                        1 if all_rows else 0, _np_ptr(out))
         if rc != 0:
             raise _err(rc)
@@ -323,7 +328,7 @@ class Session:
         u = None if u is None else np.ascontiguousarray(u, dtype=np.float64).ravel()
         if u is not None and u.size != seqs.size:
             raise ValueError("a draw for each sequence")
-        rc = lib().gbx_session_next_tokens(self.h, _np_ptr(seqs), seqs.size, _np_ptr(ids), ids.size, _np_ptr(counts),
+        rc = lib().gbx_session_next_tokens(self._open(), _np_ptr(seqs), seqs.size, _np_ptr(ids), ids.size, _np_ptr(counts),
                                            float(temperature), None if u is None else _np_ptr(u), _np_ptr(out))
         if rc != 0:
             raise _err(rc)
@@ -351,7 +356,7 @@ class Session:
                 raise ValueError("a draft count for each sequence")
         out = np.empty(tokens.shape, dtype=np.int32)
         acc = np.empty(seqs.size, dtype=np.int32)
-        rc = lib().gbx_session_verify(self.h, _np_ptr(seqs), seqs.size, _np_ptr(tokens), k,
+        rc = lib().gbx_session_verify(self._open(), _np_ptr(seqs), seqs.size, _np_ptr(tokens), k,
                                       None if draft_len is None else _np_ptr(draft_len),
                                       None if draft_logits is None else _np_ptr(draft_logits), float(temperature),
                                       None if u is None else _np_ptr(u), _np_ptr(out), _np_ptr(acc))

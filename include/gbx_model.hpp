@@ -238,7 +238,7 @@ public:
     Copies compact();
     bool known(int seq) const { return seq >= 0 && seq < (int)seqs_.size() && seqs_[seq].live; }
     int64_t length(int seq) const { return known(seq) ? seqs_[seq].length : -1; }
-    const std::vector<int32_t>& pagesOf(int seq) const { return seqs_[seq].pages; }
+    const std::vector<int32_t>& pagesOf(int seq) const { return known(seq) ? seqs_[seq].pages : none_; }
     int64_t freePages() const { return (int64_t)free_.size(); }
     int64_t pages() const { return (int64_t)refs_.size(); }
     int pageSize() const { return pageSize_; }
@@ -256,6 +256,7 @@ private:
     std::vector<int> refs_;
     std::vector<int32_t> free_;   // a heap, the lowest page first
     std::vector<Seq> seqs_;
+    std::vector<int32_t> none_;   // the pages of an unknown sequence
 };
 
 // New: cached generation.  A Session holds a paged 8-bit key/value cache of all

@@ -69,6 +69,8 @@ def test_bad_calls_are_refused(gbx):
     _refused(gbx, lambda: _attn(gbx, c, H=0), 1, "query heads")
     for scale in (0.0, -1.0, float("inf"), float("nan"), 1e-40):
         _refused(gbx, lambda: _attn(gbx, c, scale=scale), 1, "scale")
+    _refused(gbx, lambda: _attn(gbx, c, H=8192, S=1 << 20, ld=1 << 20, ld_out=1 << 20, q=1 << 45, out=1 << 46), 3, "query heads a key head")
+    _refused(gbx, lambda: gbx.attn_cached_workspace(c, B=1, S=1 << 20, H=8192, max_pages=4), 3, "query heads a key head")
     _refused(gbx, lambda: _attn(gbx, c, ld=127), 1, "ld=127")
     _refused(gbx, lambda: _attn(gbx, c, ld_out=64), 1, "ld_out=64")
     _refused(gbx, lambda: _attn(gbx, c, out=1 << 30), 1, "overlaps")

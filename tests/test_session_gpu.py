@@ -108,6 +108,10 @@ def test_steps_match_the_plain_model(gm, cuda, tmp_path, d, heads, P):
     assert s.length(seq) == 72
     s.close()
     model.close()
+    gbx = importlib.import_module("glassboxai-transformer_b200")
+    for call in (s.new, lambda: s.forward([0], [[1]]), s.compact, lambda: s.length(0)):
+        with pytest.raises(gbx.GbxError, match="closed"):
+            call()
 
 
 def test_a_prompt_is_the_forward(gm, model):
