@@ -348,12 +348,17 @@ __device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool e
     constexpr int NCH = ac_chunks(HD) / 2, pitch = ac_pitch(HD);
     float2 s[RT][8];
     // key side: this lane's tokens are 2g + (n & 1) of group n / 2
-    const uint32_t kp = kb + (n >> 1) * pitch + (n & 1) * HD + 16 * cc;
+    // columns past the head's last 16 (their query digits are 0) are read from
+    // those: 16 bytes further, a slot's last token would leave the ring
+    const uint32_t kp = kb + (n >> 1) * pitch + (n & 1) * HD;
+    uint32_t col[NCH];
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) col[ch] = min(64 * ch + 16 * cc, HD - 16);
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
         uint4 w[NCH];
 #pragma unroll
-        for (int ch = 0; ch < NCH; ++ch) w[ch] = ac_lds(kp + 2 * g * HD + 64 * ch);
+        for (int ch = 0; ch < NCH; ++ch) w[ch] = ac_lds(kp + 2 * g * HD + col[ch]);
         float2 d[RT];
         ac_dot<false, RT, ac_chunks(HD)>(d, q, w, kc);
 #pragma unroll

@@ -166,3 +166,20 @@ def test_oracle_verification_keeps_the_target_distribution():
     # five standard deviations of a count
     assert np.all(np.abs(got - p) < 5 * np.sqrt(p * (1 - p) / N))
     assert abs(acc.mean() - np.minimum(p, q).sum()) < 5 * np.sqrt(0.25 / N)
+
+
+@pytest.mark.parametrize("hd", range(16, 129, 16))
+def test_the_attention_reads_stay_in_their_slot(hd):
+    """The cached attention's shared-memory addresses, as attn_cached.cu forms them: every 16-byte read of a slot's
+    keys (lane (n, c), pair g, chunk ch) and values (lane, column block j) lies inside the slot."""
+    pitch = 16 * hd + 32
+    chunks = 2 if hd > 64 else 1
+    for n in range(8):
+        for c in range(4):
+            for g in range(8):
+                for ch in range(chunks):
+                    at = (n >> 1) * pitch + (n & 1) * hd + 2 * g * hd + min(64 * ch + 16 * c, hd - 16)
+                    assert at % 16 == 0 and at + 16 <= (n >> 1) * pitch + 16 * hd
+            for j in range(hd // 8):
+                at = c * pitch + n * 16 + 8 * j * 16
+                assert at % 16 == 0 and at + 16 <= c * pitch + 16 * hd

@@ -271,6 +271,23 @@ def pair_slack(s, q, want):
     return 2 * A * 2.0 ** -22 * vmax * np.ones_like(want)
 
 
+@pytest.mark.parametrize("hd", range(16, 129, 16))
+@pytest.mark.parametrize("rows", [1, 12, 50])
+def test_attention_of_every_head_width_uses_its_whole_ring(gbx, cuda, hd, rows):
+    """Caches long enough that every warp goes through all its slots several times."""
+    s = Setup(gbx, 16, 2, hd, 1, 4200, seed=hd)
+    q = s.rng.standard_normal((1, rows, 2, hd)).astype(np.float32)
+    kv_len, n_new = np.array([4200]), np.array([rows])
+    pick = [0, rows - 1]
+    want, tol = kv_oracle.attend(s.ref, s.table, [4200 - rows + 1], [1], q[:, :1], 8.0)
+    want1, tol1 = kv_oracle.attend(s.ref, s.table, kv_len, [1], q[:, rows - 1:], 8.0)
+    for ws in ("auto", None):
+        out, _ = run_attn(s, q, kv_len, n_new, 8.0, workspace=ws)
+        assert np.isfinite(out).all()
+        assert_attn(out[:, pick], np.concatenate([want, want1], 1), np.concatenate([tol, tol1], 1), np.ones((1, 2, 2, hd), bool))
+    assert int(s.err.item()) == 0
+
+
 @pytest.mark.parametrize("S,G,P", [(1, 1, 16), (5, 1, 32), (4, 3, 64), (40, 1, 16)])
 def test_attention_ragged_rows(gbx, cuda, S, G, P):
     """Rows past a sequence's own are left as they were; sequences without rows or tokens too."""
