@@ -428,6 +428,37 @@ __device__ __forceinline__ void ac_values(uint32_t vb, const AcDigits<RT, 2>& p,
     }
 }
 
+// A warp's finished rows base .. base + 8 RT - 1.
+template <int HD, int RT>
+__device__ __forceinline__ void ac_rows_out(const AcArgs& a, const AcUnit& u, int base, float (&l)[RT], const float2 (&o)[RT][HD / 8])
+{
+    const int lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] += __shfl_xor_sync(0xffffffffu, l[rt], 1);
+        l[rt] += __shfl_xor_sync(0xffffffffu, l[rt], 2);
+        const int r = base + 8 * rt + n;
+        if (r >= u.rows) continue;
+        const int64_t at = ac_row(a, u, r, a.ld_out) + 2 * cc;
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) {
+            const float2 v = l[rt] == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(o[rt][j].x / l[rt], o[rt][j].y / l[rt]);
+            if (a.vec_out && !a.out_lo) {
+                *reinterpret_cast<float2*>(a.out + at + 8 * j) = v;
+            } else if (a.vec_out) {
+                float2 h, lo;
+                split_value(v.x, h.x, lo.x);
+                split_value(v.y, h.y, lo.y);
+                *reinterpret_cast<float2*>(a.out + at + 8 * j) = h;
+                *reinterpret_cast<float2*>(a.out_lo + at + 8 * j) = lo;
+            } else {
+                ac_store(a, at + 8 * j, v.x);
+                ac_store(a, at + 8 * j + 1, v.y);
+            }
+        }
+    }
+}
+
 // Where the rows' partial results meet: NW partial results of R rows (one per
 // warp, or one that the warps fill together) and the CTA's own after them, in
 // the shared memory that held the ring.
@@ -952,6 +983,12 @@ __global__ void __launch_bounds__(32 * (W + 1)) attn_cached_rows_kernel(const Ac
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) l[rt] = __int_as_float(0x7fc00000);
         }
+    }
+    if (csize == 1 && a.nsplit == 1) {
+        // nobody to meet: from the registers, 32 bytes of a row at a time.  (The
+        // producer stays until its copies have landed, above.)
+        if (warp < W) ac_rows_out<HD, RT>(a, u, 8 * RT * warp, l, o);
+        return;
     }
     __syncthreads();   // the ring is done with
     AcMeet<HD, R, 1> meet(ac_smem);

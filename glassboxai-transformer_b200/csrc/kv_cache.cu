@@ -403,13 +403,14 @@ struct KvPool {
     int8_t* v;
     float* ks;
     float* vs;
-    int64_t page_bytes;    // heads * page * hd, a multiple of 256
+    int64_t page_bytes;    // heads * page * hd, a multiple of 256, at most 2^30
     int64_t pages;
     int heads, layers;
     int32_t* err;
 };
 
-// One CTA per (pair, layer, K or V): 6.0 TB/s at 600 pages of 24 layers.  A page of a layer is one contiguous
+// One CTA per (pair, layer, K or V) and, where those are fewer than four to an
+// SM, part of the page: 6.0 TB/s at 600 pages of 24 layers.  A page of a layer is one contiguous
 // run of bytes.  Before it stores, the CTA looks its target up among all
 // sources and earlier targets (n words each, from L2): a pair that would race
 // with another is left out, by every CTA alike.
@@ -419,7 +420,7 @@ kv_copy_kernel(const KvPool c, const int32_t* src, const int32_t* dst, int n)
     grid_dependency_wait();
     const int i = blockIdx.x, layer = blockIdx.y >> 1, which = blockIdx.y & 1;
     const int from = src[i], to = dst[i];
-    const bool first = blockIdx.y == 0 && threadIdx.x == 0;
+    const bool first = blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0;
     if ((uint64_t)(int64_t)from >= (uint64_t)c.pages || (uint64_t)(int64_t)to >= (uint64_t)c.pages) {
         if (first) kv_flag(c.err, GBX_KV_BAD_PAGE);
         return;
@@ -434,7 +435,11 @@ kv_copy_kernel(const KvPool c, const int32_t* src, const int32_t* dst, int n)
     int8_t* base = (which ? c.v : c.k) + (int64_t)layer * c.pages * c.page_bytes;
     const uint4* s = reinterpret_cast<const uint4*>(base + from * c.page_bytes);
     uint4* d = reinterpret_cast<uint4*>(base + to * c.page_bytes);
-    for (int64_t e = threadIdx.x; e < c.page_bytes >> 4; e += 256) d[e] = s[e];
+    const int words = (int)(c.page_bytes >> 4), part = (words + (int)gridDim.z - 1) / (int)gridDim.z;
+    const int end = min(words, ((int)blockIdx.z + 1) * part);
+#pragma unroll 4
+    for (int e = (int)blockIdx.z * part + threadIdx.x; e < end; e += 256) d[e] = s[e];
+    if (blockIdx.z) return;
     float* sc = (which ? c.vs : c.ks) + (int64_t)layer * c.pages * c.heads;
     for (int e = threadIdx.x; e < c.heads; e += 256) sc[(int64_t)to * c.heads + e] = sc[(int64_t)from * c.heads + e];
 }
@@ -586,7 +591,13 @@ extern "C" int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* 
     c.heads = h.heads;
     c.layers = h.layers;
     c.err = err_flag;
-    launch_row_kernel(kv_copy_kernel, dim3((unsigned)n, (unsigned)h.layers * 2), dim3(256), 0,
+    DeviceInfo di;
+    if (device_info(&di) != GBX_OK) return GBX_ECUDA;
+    int64_t parts = 4 * (int64_t)di.sm_count / ((int64_t)n * h.layers * 2), most = c.page_bytes / 4096;   // 256 x 16 bytes
+    if (parts > most) parts = most;
+    if (parts < 1) parts = 1;
+    if (parts > 65535) parts = 65535;
+    launch_row_kernel(kv_copy_kernel, dim3((unsigned)n, (unsigned)h.layers * 2, (unsigned)parts), dim3(256), 0,
                       reinterpret_cast<cudaStream_t>(stream), c, src, dst, n);
     return check_launch("gbx_kv_copy_pages");
 }
