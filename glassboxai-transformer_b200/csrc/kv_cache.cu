@@ -85,10 +85,12 @@ __device__ __forceinline__ KvBlock kv_block(const KvLayer& c, KvSeq q, int j)
 }
 
 // ---------------------------------------------------------------- append
+constexpr int kKvHeld = 4;   // groups of four values a lane holds between the maximum and the codes
+
 struct KvAppend {
     KvLayer c;
     KvRows r;
-    FastDiv by_heads, by_blocks;   // unit = ((b * blocks + j) * 2 + which) * heads + h
+    FastDiv by_quads, by_heads, by_blocks;   // unit = ((b * blocks + j) * 2 + which) * heads + h
     int blocks;
     uint32_t units;
 };
@@ -127,15 +129,14 @@ __device__ __forceinline__ float4 kv_load4(const float* hi, const float* lo, int
     return x;
 }
 
-// The page's scale with new values of largest size amax in, and where it grew
-// the codes of the slots before slot s0 recoded by `threads` threads, this one
+// The page's scale (old, where it holds earlier slots) with new values of
+// largest size amax in, and where it grew the codes of the slots before slot s0 recoded by `threads` threads, this one
 // the id-th.  Called by all of them, which have to meet before *scale is stored.
-__device__ __forceinline__ float kv_grow(const KvBlock& k, int8_t* codes, const float* scale, float amax, bool bad, int which, int hd,
+__device__ __forceinline__ float kv_grow(const KvBlock& k, int8_t* codes, float old, float amax, bool bad, int which, int hd,
                                          int id, int threads)
 {
     float s = kv_new_scale(amax, bad);
     if (k.s0 > 0) {
-        const float old = *scale;
         s = kv_max_scale(old, s);
         if (s != old) {   // grew, or turned NaN
             for (int e = id; e < k.s0 * hd; e += threads) {
@@ -149,9 +150,10 @@ __device__ __forceinline__ float kv_grow(const KvBlock& k, int8_t* codes, const 
 }
 
 // Few new rows per sequence (a decode step, drafts): one warp per (sequence, block, K or V, head), the
-// largest |x| of the block's new rows, the scale, the codes.  The rows are
-// read twice, the second time from L1.  Latency bounds it (length, page, rows,
-// codes one after another): 3.5 us for 32 sequences x 12 heads, 10 for 256 x 25.
+// largest |x| of the block's new rows, the scale, the codes.  The first 512
+// values are held in registers, others read again from L1.  Latency bounds it
+// (length, rows and page, scale, codes one after another): 3.3 us for 32 sequences x
+// 12 heads, 8.8 for 256 x 25.
 template <bool VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppend a)
 {
@@ -166,34 +168,43 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppend a)
     if (bad_len && lane == 0) kv_flag(c.err, GBX_KV_BAD_LEN);
     const KvBlock k = kv_block(c, q, u.j);
     if (k.n <= 0) return;
-    const int page = kv_page(c, u.b, k.page_idx);
-    if (page < 0) {
-        if (lane == 0) kv_flag(c.err, GBX_KV_BAD_PAGE);
-        return;
-    }
+    const int page = kv_page(c, u.b, k.page_idx);   // not waited for before the rows are asked for
     const int hd = c.hd;
     const float* base = a.r.hi[u.which];
     const float* hi = base + ((int64_t)u.b * c.S + k.i0) * a.r.ld + (int64_t)u.h * hd;
     const float* lo = a.r.lo[u.which] ? a.r.lo[u.which] + (hi - base) : nullptr;
+    const int quads = hd >> 2, n4 = k.n * quads;   // groups of 4 values
+    auto load = [&](int e) {
+        const int r = (int)fast_div(e, a.by_quads);
+        return kv_load4<VEC>(hi, lo, r * a.r.ld + (e - r * quads) * 4);
+    };
+    float4 held[kKvHeld];
+#pragma unroll
+    for (int i = 0; i < kKvHeld; ++i) held[i] = lane + 32 * i < n4 ? load(lane + 32 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (page < 0) {
+        if (lane == 0) kv_flag(c.err, GBX_KV_BAD_PAGE);
+        return;
+    }
     const int64_t ph = (int64_t)page * c.heads + u.h;
     int8_t* codes = (u.which ? c.v : c.k) + (ph << c.log_page) * hd;
     float* scale = (u.which ? c.vs : c.ks) + ph;
-    const int quads = hd >> 2, n4 = k.n * quads;   // groups of 4 values
     float amax = 0.0f, bad = 0.0f;
-    for (int e = lane; e < n4; e += 32) {
-        const float4 x = kv_load4<VEC>(hi, lo, (int64_t)(e / quads) * a.r.ld + (e % quads) * 4);
+    auto look = [&](float4 x) {
         amax = fmaxf(amax, kv_abs4(x));
         bad += kv_bad4(x);
-    }
+    };
+    const float old = k.s0 > 0 ? *scale : 0.0f;    // asked for before the maximum is formed
+#pragma unroll
+    for (int i = 0; i < kKvHeld; ++i) look(held[i]);
+    for (int e = lane + 32 * kKvHeld; e < n4; e += 32) look(load(e));
     amax = group_max<32>(amax);
-    const float s = kv_grow(k, codes, scale, amax, __any_sync(0xffffffffu, bad != bad), u.which, hd, lane, 32);
+    const float s = kv_grow(k, codes, old, amax, __any_sync(0xffffffffu, bad != bad), u.which, hd, lane, 32);
     __syncwarp();
     if (lane == 0) *scale = s;
     const bool live = s > 0.0f;   // false for 0 and NaN: codes 0
     const float rs = 1.0f / s;
-    for (int e = lane; e < n4; e += 32) {
-        const int r = e / quads, i = (e - r * quads) * 4, t = k.s0 + r;
-        const float4 x = kv_load4<VEC>(hi, lo, (int64_t)r * a.r.ld + i);
+    auto put = [&](int e, float4 x) {
+        const int r = (int)fast_div(e, a.by_quads), i = (e - r * quads) * 4, t = k.s0 + r;
         const uint32_t q4 = live ? kv_codes4(x, s, rs) : 0u;
         if (u.which) {
             int8_t* p = codes + ((t >> 4) * hd + i) * 16 + (t & 15);
@@ -202,7 +213,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppend a)
         } else {
             *reinterpret_cast<uint32_t*>(codes + t * hd + i) = q4;
         }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kKvHeld; ++i)
+        if (lane + 32 * i < n4) put(lane + 32 * i, held[i]);
+    for (int e = lane + 32 * kKvHeld; e < n4; e += 32) put(e, load(e));
 }
 
 // Many new rows: one CTA per (sequence, block, K or V, head), a warp for every
@@ -290,7 +305,7 @@ __global__ void __launch_bounds__(512) kv_append_pages_kernel(const KvAppend a)
         amax = fmaxf(amax, s_max[w]);
         bad += s_bad[w];
     }
-    const float s = kv_grow(k, codes, scale, amax, bad != bad, u.which, hd, threadIdx.x, blockDim.x);
+    const float s = kv_grow(k, codes, k.s0 > 0 ? *scale : 0.0f, amax, bad != bad, u.which, hd, threadIdx.x, blockDim.x);
     __syncthreads();   // every thread has read the old scale, and recoded what it recodes
     if (threadIdx.x == 0) *scale = s;
     if (col >= hd) return;
@@ -528,12 +543,13 @@ extern "C" int gbx_kv_append(const gbx_kv_cache* cache_host, int layer, const in
     a.r.ld = ld;
     a.by_heads = make_fastdiv(c.heads);
     a.by_blocks = make_fastdiv(blocks);
+    a.by_quads = make_fastdiv(c.hd / 4);
     a.blocks = blocks;
     a.units = (uint32_t)units;
     const bool vec = aligned16(k_hi) && aligned16(v_hi) && aligned16(k_lo) && aligned16(v_lo) && ld % 4 == 0;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     // Whole pages pay for a CTA each: 256 rows of 25 heads x 64 at 16 rows a sequence and
-    // 64 to a page take 13 us by rows and 27 by pages, at 32 rows 27 and 28; 64 rows at 16 to a
+    // 64 to a page take 13 us by rows and 27 by pages, at 32 rows 26 and 28; 64 rows at 16 to a
     // page 34 and 22, 8 prompts of 1024 rows at 64 101 and 33.
     if (S < 32 || S < P) {
         const dim3 grid((unsigned)((units + 7) / 8));

@@ -37,7 +37,6 @@ namespace gbx {
 
 constexpr int kVfMaxDraft = 256;
 constexpr int kVfQuads = 2;      // 16-byte loads of a lane in one unit of A
-constexpr int kVfAhead = 2;      // units in flight
 
 // A warp's run of the vocabulary, and a lane's neighbouring entries of it (odd:
 // the lanes' doubles then lie in different banks).
@@ -144,11 +143,14 @@ struct VfExp {
 };
 
 // C: CTAs of a cluster.
-// W: warps of a CTA.  KEEP: part C holds the exponentials it sums in shared memory.
-template <int C, int W, bool KEEP>
+// W: warps of a CTA.
+enum { VF_GREEDY, VF_AGAIN, VF_KEEP };   // sampling: part C forms its exponentials again, or keeps them in shared memory
+template <int C, int W, int MODE>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const VfArgs a)
 {
     constexpr int kVfRuns = C * W, kVfThreads = 32 * W;
+    constexpr bool GREEDY = MODE == VF_GREEDY, KEEP = MODE == VF_KEEP;
+    constexpr int kVfAhead = W == 8 ? 3 : 2;   // units of A in flight
     grid_dependency_wait();
     vf_arrive();   // awaited before the first write into another CTA
     extern __shared__ __align__(16) float2 s_warp[];                                            // [rows][warps]
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
     const bool bad_len = len < 0 || len > n;
     if (bad_len) len = 0;
     const float* tl = a.logits + b * (n + 1) * (int64_t)V;
-    const float* dl = a.draft_logits && !a.greedy ? a.draft_logits + b * (int64_t)n * V : nullptr;
+    const float* dl = a.draft_logits && !GREEDY ? a.draft_logits + b * (int64_t)n * V : nullptr;
     const int32_t* ids = a.draft_ids + b * n;
     // this warp's run of a row in C
     const int run = vf_run(V, kVfRuns), seg = vf_seg(run);
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
     // ---------------------------------------------------- A
     // Here a warp's share of a row is a run of 16-byte quads, which start at the
     // row's own first aligned entry; the up to six entries around them are warp
-    // 0's.  Unit u: pass u % passes (64 quads) of row u / passes, the next two
+    // 0's.  Unit u: pass u % passes (64 quads) of row u / passes, the next few
     // units' loads in flight while one is worked on.
     constexpr int N = kVfQuads, Q = 32 * N;
     const int share = ((V >> 2) + kVfRuns) / kVfRuns, passes = (share + Q - 1) / Q;
@@ -214,13 +216,13 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
 #pragma unroll
     for (int i = 0; i < kVfAhead; ++i) fetch_next(next[i]);
     // what B and C need from memory, asked for meanwhile
-    const double u_next = a.greedy ? 0.0 : a.uniforms[b * (n + 1) + n];
+    const double u_next = GREEDY ? 0.0 : a.uniforms[b * (n + 1) + n];
     int d_mine = -1;
     float tl_mine = 0.0f, dl_mine = 0.0f;
     double u_mine = 0.0;
     if (tid < len) {
         d_mine = ids[tid];
-        if (!a.greedy) u_mine = a.uniforms[b * (n + 1) + tid];
+        if (!GREEDY) u_mine = a.uniforms[b * (n + 1) + tid];
         if ((unsigned)d_mine < (unsigned)V) {
             tl_mine = tl[(int64_t)tid * V + d_mine];
             if (dl) dl_mine = dl[(int64_t)tid * V + d_mine];
@@ -228,17 +230,20 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
     }
     if (tid < 128) s_root[tid] = exp2(tid * (1.0 / 128.0));
     if (tid == 0) s_dec = len;
-    for (int k = 0; k < nrows; ++k) {
-        float m = -INFINITY, s = 0.0f;
-        int at = 0x7fffffff;
-        bool nan = false;
-        for (int pass = 0; pass < passes; ++pass) {
-            const Unit u = next[0];
-            next[0] = next[1];
-            fetch_next(next[1]);
-            static_assert(N == 2 && kVfAhead == 2, "as written out here");
+    float m = -INFINITY, s = 0.0f;
+    int at = 0x7fffffff, k = 0, pass = 0;
+    bool nan = false;
+    const int units = nrows * passes;
+    for (int u0 = 0; u0 < units; u0 += kVfAhead) {
+        // unrolled, so that each unit in flight has registers of its own: moving
+        // one that is still loading would wait for it
+#pragma unroll
+        for (int i = 0; i < kVfAhead; ++i) {
+            if (u0 + i >= units) continue;
+            const Unit& u = next[i];
+            static_assert(N == 2, "as written out here");
             const float v[4 * N + 1] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w, u.v[1].x, u.v[1].y, u.v[1].z, u.v[1].w, u.x};
-            if (a.greedy) {
+            if (GREEDY) {
 #pragma unroll
                 for (int e = 0; e <= 4 * N; ++e) {
                     const int j = e == 4 * N ? u.jx : u.j + 128 * (e >> 2) + (e & 3);
@@ -263,22 +268,30 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
                 s = fmaf(s, vf_exp2(fmaf(m, a.c2, -base)), t.x + t.y);             // m = -inf: 0
                 m = bm;
             }
+            fetch_next(next[i]);
+            if (++pass < passes) continue;
+            float2 st;
+            if (GREEDY) {
+                st = vf_reduce<32>(make_float2(nan ? __int_as_float(0x7fc00000) : m, __int_as_float(at)), a.c2, 1);
+            } else {
+                const float wm = group_max<32>(m), base = wm == -INFINITY ? 0.0f : wm;
+                st = make_float2(wm, group_sum<32>(s * vf_exp2((m - base) * a.c2)));
+            }
+            if (lane == 0) s_warp[k * W + warp] = st;
+            ++k;
+            pass = 0;
+            m = -INFINITY;
+            s = 0.0f;
+            at = 0x7fffffff;
+            nan = false;
         }
-        float2 st;
-        if (a.greedy) {
-            st = vf_reduce<32>(make_float2(nan ? __int_as_float(0x7fc00000) : m, __int_as_float(at)), a.c2, 1);
-        } else {
-            const float wm = group_max<32>(m), base = wm == -INFINITY ? 0.0f : wm;
-            st = make_float2(wm, group_sum<32>(s * vf_exp2((m - base) * a.c2)));
-        }
-        if (lane == 0) s_warp[k * W + warp] = st;
     }
     __syncthreads();
     vf_wait();   // the other CTAs run
     // this CTA's part of each row, to every CTA
     for (int i = tid; i < (nrows * W + 31 & ~31); i += kVfThreads) {
         const int k = i / W, w = i % W;
-        const float2 t = vf_reduce<W>(k < nrows ? s_warp[i] : make_float2(-INFINITY, 0.0f), a.c2, a.greedy);
+        const float2 t = vf_reduce<W>(k < nrows ? s_warp[i] : make_float2(-INFINITY, 0.0f), a.c2, GREEDY);
         if (k < nrows)
             for (uint32_t p = w; p < C; p += W) vf_push(s_part + k * C + rank, p, t);
     }
@@ -287,8 +300,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
     // the whole rows; x NaN: the row gives no distribution
     for (int i = tid; i < (nrows * C + 31 & ~31); i += kVfThreads) {
         const int k = i / C;
-        float2 t = vf_reduce<C>(k < nrows ? s_part[i] : make_float2(-INFINITY, 0.0f), a.c2, a.greedy);
-        if (fabsf(t.x) == INFINITY || (!a.greedy && t.y != t.y)) t.x = __int_as_float(0x7fc00000);
+        float2 t = vf_reduce<C>(k < nrows ? s_part[i] : make_float2(-INFINITY, 0.0f), a.c2, GREEDY);
+        if (fabsf(t.x) == INFINITY || (!GREEDY && t.y != t.y)) t.x = __int_as_float(0x7fc00000);
         if (k < nrows && i % C == 0) s_stat[k] = t;
     }
     __syncthreads();
@@ -299,7 +312,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
         const bool known = (unsigned)d_mine < (unsigned)V;
         if (!known && rank == 0) kv_flag(a.err, GBX_VERIFY_BAD_ID);
         bool ok = st.x == st.x && known;
-        if (ok && a.greedy) {
+        if (ok && GREEDY) {
             ok = d_mine == __float_as_int(st.y);
         } else if (ok) {
             double q = 1.0;
@@ -326,15 +339,15 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
         }
     }
     if (rank == 0) {
-        const int next = a.greedy && !bad ? __float_as_int(sp.y) : -1;
+        const int next = GREEDY && !bad ? __float_as_int(sp.y) : -1;
         for (int i = tid; i <= n; i += kVfThreads)
-            if (i != acc || a.greedy || bad) a.out_ids[b * (n + 1) + i] = i < acc ? ids[i] : i == acc ? next : -1;
+            if (i != acc || GREEDY || bad) a.out_ids[b * (n + 1) + i] = i < acc ? ids[i] : i == acc ? next : -1;
         if (tid == 0) {
             a.n_accepted[b] = acc;
             if (bad) kv_flag(a.err, GBX_VERIFY_BAD_ROW);
         }
     }
-    if (a.greedy || bad) return;   // every CTA of the cluster alike
+    if (GREEDY || bad) return;   // every CTA of the cluster alike
 
     // ---------------------------------------------------- C
     const float* px = tl + (int64_t)acc * V;
@@ -467,10 +480,10 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
 template <int C, int W>
 static int vf_launch(const VfArgs& a, int64_t B, const DeviceInfo& di, cudaStream_t s)
 {
-    const size_t stats = vf_stats(a.n, C, W) + 8, kept = a.greedy ? 0 : vf_kept(a.vocab, C, W);
-    const bool keep = stats + kept + 8192 <= (size_t)di.max_smem_optin;
+    const size_t stats = vf_stats(a.n, C, W) + 8, kept = vf_kept(a.vocab, C, W);
+    const bool keep = !a.greedy && stats + kept + 8192 <= (size_t)di.max_smem_optin;
     const size_t smem = stats + (keep ? kept : 0);
-    auto k = keep ? verify_kernel<C, W, true> : verify_kernel<C, W, false>;
+    auto k = a.greedy ? verify_kernel<C, W, VF_GREEDY> : keep ? verify_kernel<C, W, VF_KEEP> : verify_kernel<C, W, VF_AGAIN>;
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
         (C > 8 && cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
         return check_launch("gbx_verify_tokens: launch attributes");
