@@ -25,11 +25,11 @@
 //
 // The fp64 exponential is table-driven (P. T. P. Tang, "Table-driven
 // implementation of the exponential function in IEEE floating-point
-// arithmetic", 1989): with t = 128 (x - m) / (T ln 2), one FMA of the logit,
+// arithmetic", 1989): with t = 128 (x - m) / (T ln 2),
 // k = rint(t) and r = t - k, e^((x - m) / T) = 2^(k/128) e^(r ln 2 / 128), the
 // second factor by its Taylor polynomial of degree 4 (|r ln 2 / 128| < 0.0028:
 // remainder below 1.3e-15), the 128 roots computed into shared memory by
-// exp2(): nine fp64 instructions where the fp64 pipe is what bounds C.
+// exp2(): ten fp64 instructions where the fp64 pipe is what bounds C.
 #include "gbx_common.cuh"
 #include "kv_cache.cuh"
 
@@ -118,17 +118,18 @@ __device__ __forceinline__ float2 vf_reduce(float2 v, float c2, int greedy)
 }
 
 // The exponential of one distribution (see the header): e^((x - m) / T) of a
-// logit x; 0 below e^-700.
+// logit x; 0 below e^-700.  x - m is formed first: as one FMA with m c rounded,
+// a row of nothing but the lowest float would lose its equal entries.
 struct VfExp {
-    double c, d;          // t = x c + d
+    double m, c;          // t = (x - m) c
     const double* root;   // 2^(i/128)
-    __device__ __forceinline__ VfExp(double m, double inv_t, const double* roots)
-        : c(inv_t * 184.6649652337873), d(-m * (inv_t * 184.6649652337873)), root(roots)
+    __device__ __forceinline__ VfExp(double m_, double inv_t, const double* roots)
+        : m(m_), c(inv_t * 184.6649652337873), root(roots)
     {
     }
     __device__ __forceinline__ double operator()(float x) const
     {
-        const double t = fma((double)x, c, d);
+        const double t = ((double)x - m) * c;
         const double big = t + 6755399441055744.0;       // 1.5 2^52: k in the low word
         const double r = t - (big - 6755399441055744.0);
         const int k = __double2loint(big);
@@ -257,15 +258,16 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
                 float bm = fmaxf(m, v[4 * N]);
 #pragma unroll
                 for (int e = 0; e < 4 * N; ++e) bm = fmaxf(bm, v[e]);
-                const float base = (bm == -INFINITY ? 0.0f : bm) * a.c2;
+                // the maximum is taken off first: a mask of the lowest float times c2 would overflow
+                const float base = bm == -INFINITY ? 0.0f : bm;
                 const float2 by = splat2(a.c2), less = splat2(-base);
-                float2 t = make_float2(vf_exp2(fmaf(v[4 * N], a.c2, -base)), 0.0f);   // a NaN makes the sum NaN
+                float2 t = make_float2(vf_exp2((v[4 * N] - base) * a.c2), 0.0f);   // a NaN makes the sum NaN
 #pragma unroll
                 for (int e = 0; e < 4 * N; e += 2) {
-                    const float2 y = __ffma2_rn(make_float2(v[e], v[e + 1]), by, less);
+                    const float2 y = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), less), by);
                     t = __fadd2_rn(t, make_float2(vf_exp2(y.x), vf_exp2(y.y)));
                 }
-                s = fmaf(s, vf_exp2(fmaf(m, a.c2, -base)), t.x + t.y);             // m = -inf: 0
+                s = fmaf(s, vf_exp2((m - base) * a.c2), t.x + t.y);                // m = -inf: 0
                 m = bm;
             }
             fetch_next(next[i]);
@@ -518,7 +520,8 @@ extern "C" int gbx_verify_tokens(const float* logits, const float* draft_logits,
 {
     if (B < 0 || n_draft < 0 || vocab <= 0)
         return set_error(GBX_EINVAL, "gbx_verify_tokens: B=%lld n_draft=%d vocab=%d", (long long)B, n_draft, vocab);
-    if (!(temperature < INFINITY)) return set_error(GBX_EINVAL, "gbx_verify_tokens: temperature %g", temperature);
+    // its reciprocal has to be an fp32 number
+    if (!(temperature < 1e38)) return set_error(GBX_EINVAL, "gbx_verify_tokens: temperature %g", temperature);
     if (n_draft > kVfMaxDraft) return set_error(GBX_ERANGE, "gbx_verify_tokens: n_draft=%d (at most %d)", n_draft, kVfMaxDraft);
     if (B > 0x7fffffffLL / 16) return set_error(GBX_ERANGE, "gbx_verify_tokens: B=%lld", (long long)B);
     if (B == 0) return GBX_OK;

@@ -586,7 +586,7 @@ int64_t gbx_attn_cached_workspace(const gbx_kv_cache* cache_host, int B, int S, 
  * so the tokens are distributed as the target's own.  temperature <= 0.01:
  * drafts are accepted while they are the row's argmax (the first maximum, as
  * gbx_select_tokens), the next token is the argmax; uniforms and draft_logits
- * are not read.  -inf logits are tokens of probability 0.
+ * are not read; it has to be below 1e38.  -inf logits are tokens of probability 0.
  *   n_accepted[b]  drafts accepted
  *   out_ids[b][.]  n_draft + 1 entries: the accepted drafts, the next token, -1s
  * A row that gives no distribution (GBX_VERIFY_BAD_ROW) ends its sequence

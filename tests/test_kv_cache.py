@@ -183,3 +183,8 @@ def test_the_attention_reads_stay_in_their_slot(hd):
             for j in range(hd // 8):
                 at = c * pitch + n * 16 + 8 * j * 16
                 assert at % 16 == 0 and at + 16 <= c * pitch + 16 * hd
+
+
+def test_temperatures_without_an_fp32_reciprocal_are_refused(gbx):
+    for t in (1e38, 1e300):
+        _refused(gbx, lambda: gbx.verify_tokens(16, 16, 16, 16, temperature=t, B=1, n_draft=1, vocab=4, uniforms=16), 1, "temperature")

@@ -154,3 +154,27 @@ def test_a_row_without_drafts_is_a_plain_sample(gbx, cuda):
     sel = torch.empty(B, dtype=torch.int32, device="cuda")
     gbx.select_tokens(dev(logits[:, 0]), sel, rows=B, vocab=V, temperature=0.9, uniforms=dev(u[:, 0].copy()))
     assert (sel.cpu().numpy() == out[:, 0]).mean() > 0.9
+
+
+@pytest.mark.parametrize("B,V,T", [(3, 50257, 0.7), (40, 50257, 1.0), (5, 700, 1.3), (3, 140001, 0.5), (4, 5000, 0.05), (3, 900, 1e30)])
+def test_masks_of_the_lowest_float_and_large_logits(gbx, cuda, B, V, T):
+    """Most of the vocabulary masked by the lowest float, a row of nothing else (uniform), and logits far from 0."""
+    import torch
+    rng = np.random.default_rng(V)
+    n, low = 3, np.finfo(np.float32).min
+    logits, draft, ids, u = inputs(rng, B, n, V, T)
+    masked = rng.random((B, 1, V)) < 0.97
+    masked[:, :, 5] = False
+    logits[np.broadcast_to(masked, logits.shape)] = low
+    draft[np.broadcast_to(masked, draft.shape)] = low
+    ids = (draft + 0.5 * rng.standard_normal(draft.shape)).argmax(-1)
+    logits[0, 1] = low
+    draft[0, 1] = low
+    logits[1] = np.where(masked[1], low, np.float32(1000) + logits[1])
+    draft[1] = np.where(masked[1], low, np.float32(1000) + draft[1])
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for d in (draft, None):
+        want, wacc = kv_oracle.verify(logits, d, ids, np.full(B, n), T, u)
+        got, acc = run(gbx, logits, d, ids, None, T, u, err=err)
+        assert np.array_equal(acc, wacc) and np.array_equal(got, want)
+    assert int(err.item()) == 0
