@@ -598,3 +598,33 @@ def test_the_same_call_gives_the_same_bits(gbx, cuda, tokens_, cut):
     for _ in range(5):
         again, _ = run_attn(s, q, [tokens_], [1], 8.0)
         assert np.array_equal(first, again)
+
+
+@pytest.mark.parametrize("hd,S", [(64, 1), (64, 4), (32, 20), (128, 20)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_from_zero(gbx, cuda, hd, S, sign):
+    """Rows whose one best key is ahead by more than any rounding, at scores of 10^2 to 10^15 in size, above and
+    below 0: they return that key's value, to 2^-19 of it (the weight's fixed point half of 2^-23 over a ratio of value
+    scales of at least 1/3; fewer than 20 fp32 roundings and two approximations of 2^-22)."""
+    heads, L = 2, 300
+    s = Setup(gbx, 16, heads, hd, 1, L, seed=hd + S)
+    rng = np.random.default_rng(17)
+    best = rng.integers(0, L - S, (S, heads))
+    big = 10.0 ** rng.uniform(2, 15, (S, heads))
+    s.ref.scale[0][:] = np.float32(1 / 60)
+    q = np.zeros((1, S, heads, hd), np.float32)
+    want = np.zeros(q.shape)
+    for h in range(heads):
+        for i in range(S):
+            # key columns i mod hd, one to a row: its best token is ahead (or least behind) by half
+            c = i % hd
+            for t in range(L):
+                s.ref.codes[0][s.table[0, t // 16], h, t % 16, c] = 60 if sign > 0 else 120
+            t = int(best[i, h])
+            s.ref.codes[0][s.table[0, t // 16], h, t % 16, c] = 120 if sign > 0 else 60
+            q[0, i, h, c] = sign * big[i, h]
+            want[0, i, h] = s.ref.codes[1][s.table[0, t // 16], h, t % 16].astype(np.float64) * s.ref.scale[1][s.table[0, t // 16], h]
+    s.upload()
+    out, _ = run_attn(s, q, [L], [S], 1.0)[:2]
+    err = np.abs(out.astype(np.float64) - want)
+    assert np.all(err <= np.abs(want) * 2.0 ** -19 + 1e-30), f"{np.argwhere(err > np.abs(want) * 2.0 ** -19)[:5].tolist()}"
