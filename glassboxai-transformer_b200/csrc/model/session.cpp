@@ -184,6 +184,20 @@ struct OnDevice {   // the model's device current, for a scope
     }
 };
 
+// Puts a page table back as it was unless the call came to its end: the pages a
+// step copied from, or would have written behind the sequences' ends, are
+// still theirs.
+struct Restore {
+    PageTable& table;
+    PageTable saved;
+    bool done = false;
+    explicit Restore(PageTable& t) : table(t), saved(t) {}
+    ~Restore()
+    {
+        if (!done) table = std::move(saved);
+    }
+};
+
 }  // namespace
 
 struct Session::Impl {
@@ -257,6 +271,10 @@ bool Session::check(const std::vector<int>& seqs, const std::vector<int>& ids, c
 {
     err_.clear();
     if (!ok_) return fail("session: not open");
+    const gbx_kv_cache& c = impl_->cache;
+    if (!model_.isModelLoaded() || model_.getNumLayers() != c.layers || model_.getNumHeads() != c.heads ||
+        model_.getEmbedDim() != c.heads * c.hd)
+        return fail("session: the model is not the one it was opened on");
     if (seqs.empty() || seqs.size() != counts.size()) return fail("session: a count for each of at least one sequence");
     int64_t all = 0;
     *S = 0;
@@ -278,13 +296,13 @@ bool Session::check(const std::vector<int>& seqs, const std::vector<int>& ids, c
     return true;
 }
 
-// Appends and runs the model; the logits stay in the model's buffer.
+// Appends and runs the model; the logits stay in the model's buffer.  The caller
+// puts the page table back if this, or what it does with the logits, fails.
 bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, bool allRows,
                    const std::vector<int>& padded, int S)
 {
     Impl& m = *impl_;
     OnDevice on(m.device);
-    PageTable saved = table_;   // put back if the step fails: the pages it copied from are untouched
     std::vector<int64_t> before;
     bool even = true, empty = true;
     for (size_t i = 0; i < seqs.size(); ++i) {
@@ -322,7 +340,6 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
     }
     if (!good) {
         cudaStreamSynchronize(m.stream);
-        table_ = std::move(saved);
         return fail(std::string("session: preparing the step failed: ") + gbx_last_error());
     }
     TransformerModel::CachedStep st;
@@ -338,11 +355,7 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
     st.even = even;
     st.fresh = even && empty;
     st.allRows = allRows;
-    if (!model_.runForward(padded, B, nullptr, &st)) {
-        table_ = std::move(saved);
-        return fail(model_.lastError());
-    }
-    return true;
+    return model_.runForward(padded, B, nullptr, &st) || fail(model_.lastError());
 }
 
 std::vector<float> Session::forward(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts,
@@ -351,7 +364,9 @@ std::vector<float> Session::forward(const std::vector<int>& seqs, const std::vec
     int S = 0;
     std::vector<int> padded;
     std::vector<float> out;
-    if (!check(seqs, ids, counts, &S, &padded) || !step(seqs, ids, counts, allRows, padded, S)) return out;
+    if (!check(seqs, ids, counts, &S, &padded)) return out;
+    Restore table(table_);
+    if (!step(seqs, ids, counts, allRows, padded, S)) return out;
     OnDevice on(impl_->device);
     const size_t V = (size_t)model_.getVocabSize();
     const float* logits = model_.deviceLogits();
@@ -371,6 +386,7 @@ std::vector<float> Session::forward(const std::vector<int>& seqs, const std::vec
         fail("session: device-to-host copy of the logits failed");
         out.clear();
     }
+    table.done = good;
     return out;
 }
 
@@ -392,6 +408,7 @@ std::vector<int> Session::nextTokens(const std::vector<int>& seqs, const std::ve
         fail("session: cudaMalloc failed");
         return out;
     }
+    Restore table(table_);
     if (!step(seqs, ids, counts, false, padded, S)) return out;
     double* du = (double*)m.select.p;
     int32_t* dids = (int32_t*)(du + B);
@@ -405,6 +422,7 @@ std::vector<int> Session::nextTokens(const std::vector<int>& seqs, const std::ve
         return out;
     }
     out.assign(got.begin(), got.end());
+    table.done = true;
     return out;
 }
 
@@ -451,7 +469,7 @@ bool Session::verify(const std::vector<int>& seqs, const std::vector<int>& ids, 
     const size_t offLogits = du.size() * 8, offIds = offLogits + logitBytes, offLens = offIds + cut.size() * 4,
                  offOut = offLens + B * 4, offAcc = offOut + B * (size_t)S * 4;
     if (!m.select.ensure(offAcc + B * 4)) return fail("session: cudaMalloc failed");
-    PageTable saved = table_;
+    Restore table(table_);
     std::vector<int64_t> before;
     for (int s : seqs) before.push_back(table_.length(s));
     if (!step(seqs, given, counts, true, padded, S)) return false;
@@ -473,16 +491,15 @@ bool Session::verify(const std::vector<int>& seqs, const std::vector<int>& ids, 
            cudaMemcpyAsync(acc.data(), p + offAcc, B * 4, cudaMemcpyDeviceToHost, m.stream) == cudaSuccess &&
            cudaMemcpyAsync(&bits, m.err, 4, cudaMemcpyDeviceToHost, m.stream) == cudaSuccess &&
            cudaStreamSynchronize(m.stream) == cudaSuccess;
-    if (!good || bits) {
-        table_ = std::move(saved);
+    if (!good || bits)
         return fail(good ? std::string("session: a logits row gives no distribution") : std::string("session: verification failed: ") + gbx_last_error());
-    }
     outIds->assign(B * n1, -1);
     accepted->assign(acc.begin(), acc.end());
     for (size_t b = 0; b < B; ++b) {
         for (int j = 0; j < S; ++j) (*outIds)[b * n1 + j] = out[b * S + j];
         table_.truncate(seqs[b], before[b] + 1 + acc[b]);
     }
+    table.done = true;
     return true;
 }
 

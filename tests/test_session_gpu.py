@@ -301,3 +301,18 @@ def test_two_sessions_of_one_model_take_turns(gm, model):
     for tok in rng.integers(0, 700, 5):
         got, _, want = a.forward([x], [[tok]]), b.forward([y], [[tok]]), alone.forward([z], [[tok]])
         assert np.array_equal(got.view(np.uint32), want.view(np.uint32))
+
+
+def test_a_verification_that_fails_after_its_forward_is_undone(gm, model, cuda):
+    gbx = importlib.import_module("glassboxai-transformer_b200")
+    s = gm.Session(model, 6, 16)
+    x = s.new()
+    s.forward([x], [[1, 2, 3]])
+    y = s.fork(x)                       # shares the page that the step writes to
+    free = s.free_pages()
+    for t in (float("inf"), 1e300):
+        with pytest.raises(gbx.GbxError, match="temperature"):
+            s.verify([x], [[4, 5, 6]], temperature=t, u=np.full((1, 3), 0.5))
+        assert s.length(x) == s.length(y) == 3 and s.free_pages() == free
+    out, acc = s.verify([x], [[4, 5, 6]])
+    assert s.length(x) == 4 + acc[0] and s.length(y) == 3
