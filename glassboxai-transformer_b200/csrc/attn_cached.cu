@@ -857,13 +857,16 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
 // go through the same steps, whose copies a warp of its own keeps in flight in
 // one ring.  The int8 tensor path bounds it: 16 rows x 64 tokens of width 64 are
 // 96 instructions of 8 cycles, and half as many exponentials as those take.  2 x
-// 512 rows x 16 heads over 2048 tokens take 59 us with 31% of the tensor cycles
+// 512 rows x 16 heads over 2048 tokens take 60 us with 31% of the tensor cycles
 // used: two warps to a scheduler do not cover each other's dependent
 // instructions.  Measured and not kept: 2 or 8 warps to a CTA (63 and 67 us),
 // two CTAs that split the steps (79), the next step's scores formed beside this
 // one's softmax (244 registers, 82 us).
+// The launch bound is one warp more than there are, which makes the register limit
+// 168: from 169 on an SM's four schedulers take 8 warps, one CTA, instead of 12
+// (width 32: 1038 us with an unbounded kernel's schedule, 970 with this one).
 template <int HD, int W, int NS>
-__global__ void __launch_bounds__(32 * (W + 1)) attn_cached_rows_kernel(const AcArgs a)
+__global__ void __launch_bounds__(32 * (W + 2), HD <= 64 ? 2 : 1) attn_cached_rows_kernel(const AcArgs a)
 {
     grid_dependency_wait();
     constexpr int RT = 2, R = 8 * RT * W, T = 32 * (W + 1);
@@ -877,7 +880,8 @@ __global__ void __launch_bounds__(32 * (W + 1)) attn_cached_rows_kernel(const Ac
     uint32_t rank, csize;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
-    const uint32_t cid = blockIdx.x >> (31 - __clz((int)csize));
+    uint32_t cid;
+    asm("mov.u32 %0, %%clusterid.x;" : "=r"(cid));
     const uint32_t unit = fast_div(cid, a.by_nsplit);
     const int split = (int)(cid - unit * a.nsplit);
     bool bad_len;
@@ -1065,13 +1069,24 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bo
     // the workspace, which costs a second launch and is taken where it at least
     // doubles the CTAs.
     const int64_t steps = ((int64_t)max_pages * c->page + kAcTile - 1) / kAcTile;
-    const int64_t per_sm = many ? (c->hd <= 64 ? 3 : c->hd <= 96 ? 2 : 1) : (int64_t)((size_t)kAcSmemPerSM / (kAcWarps * kAcSlots * 4 * ac_pitch(c->hd) + 2048));
+    // Registers bound the rows kernel (168 to a thread up to width 64, 255 beyond).
+    const int64_t per_sm = many ? (c->hd <= 64 ? 2 : 1) : (int64_t)((size_t)kAcSmemPerSM / (kAcWarps * kAcSlots * 4 * ac_pitch(c->hd) + 2048));
     const int64_t resident = di.sm_count * per_sm;
     int64_t share = resident / p->units;
     if (share > (steps + W - 1) / W) share = (steps + W - 1) / W;
     p->csize = 1;
     p->nsplit = 1;
     while (p->csize < kAcMaxCluster && 2 * p->csize <= share) p->csize *= 2;
+    // Rows kernels, which stay on the chip longer, also take the sizes between, where
+    // up to c - 1 CTA places left over in each of the 8 GPCs do not cost a second wave
+    // (64 rows over 3000 tokens: 80 units in threes 36 us against 49 in twos, 42 in sixes
+    // 22.6 against 29.0 in fours; 96 in threes would take 56 against 49).
+    if (many)
+        for (int c = kAcMaxCluster - 1; c > p->csize; --c)
+            if (c <= share && p->units * c + 8 * (c - 1) <= resident) {
+                p->csize = c;
+                break;
+            }
     if (share >= 2 * kAcMaxCluster && cut) {
         int64_t best = 0;
         for (int cs = kAcMaxCluster; cs >= 1; cs /= 2) {

@@ -628,3 +628,20 @@ def test_scores_far_from_zero(gbx, cuda, hd, S, sign):
     out, _ = run_attn(s, q, [L], [S], 1.0)[:2]
     err = np.abs(out.astype(np.float64) - want)
     assert np.all(err <= np.abs(want) * 2.0 ** -19 + 1e-30), f"{np.argwhere(err > np.abs(want) * 2.0 ** -19)[:5].tolist()}"
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("steps", [2, 3, 5, 6, 7, 9])
+def test_rows_shared_by_any_number_of_blocks(gbx, cuda, hd, steps):
+    """Prompts whose 64-token steps leave a row block to 2 .. 8 CTAs, with a last step that is not full."""
+    L, S, B = 64 * steps - 17, 70, 2
+    s = Setup(gbx, 64, 2, hd, B, 64 * steps, seed=steps)
+    q = np.random.default_rng(steps).standard_normal((B, S, 4, hd)).astype(np.float32)
+    kv_len, n_new = [L, L - 40], [S, 33]
+    want, tol = kv_oracle.attend(s.ref, s.table, kv_len, n_new, q, 9.0)
+    live = ~np.isnan(want)
+    for ws in ("auto", None):
+        out, _ = run_attn(s, q, kv_len, n_new, 9.0, workspace=ws)
+        assert_attn(out, want, tol, live)
+        assert np.isnan(out[~live]).all()
+    assert int(s.err.item()) == 0
