@@ -1069,9 +1069,12 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bo
     // the workspace, which costs a second launch and is taken where it at least
     // doubles the CTAs.
     const int64_t steps = ((int64_t)max_pages * c->page + kAcTile - 1) / kAcTile;
-    // Registers bound the rows kernel (168 to a thread up to width 64, 255 beyond).
-    const int64_t per_sm = many ? (c->hd <= 64 ? 2 : 1) : (int64_t)((size_t)kAcSmemPerSM / (kAcWarps * kAcSlots * 4 * ac_pitch(c->hd) + 2048));
-    const int64_t resident = di.sm_count * per_sm;
+    // CTAs resident on an SM.  Registers bound the rows kernel (168 to a thread up to
+    // width 64, 255 beyond) and, with the rings' shared memory, the other (8 rows: 90 at
+    // width 16, 108 up to 64, 147 beyond; 16 rows: 128, 168 and 255).
+    const int64_t by_regs = many ? (c->hd <= 64 ? 2 : 1) : (c->hd <= 16 ? 5 : c->hd <= 64 ? 4 : 3) - (p->rt == 2);
+    const int64_t by_smem = (int64_t)((size_t)kAcSmemPerSM / (kAcWarps * kAcSlots * 4 * ac_pitch(c->hd) + 2048));
+    const int64_t resident = di.sm_count * (many || by_regs < by_smem ? by_regs : by_smem);
     int64_t share = resident / p->units;
     if (share > (steps + W - 1) / W) share = (steps + W - 1) / W;
     p->csize = 1;
