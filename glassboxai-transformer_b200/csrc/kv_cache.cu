@@ -425,8 +425,8 @@ struct KvPool {
 };
 
 // One CTA per (pair, layer, K or V) and, where those are fewer than four to an
-// SM, part of the page: 6.0 TB/s at 600 pages of 24 layers.  A page of a layer is one contiguous
-// run of bytes.  Before it stores, the CTA looks its target up among all
+// SM, part of the page: 600 pages of 24 layers in 287 us, 6.6 TB/s, two pages of 5 in
+// 2.8 (8.2 whole).  A page of a layer is one contiguous run of bytes.  Before it stores, the CTA looks its target up among all
 // sources and earlier targets (n words each, from L2): a pair that would race
 // with another is left out, by every CTA alike.
 __global__ void __launch_bounds__(256)
