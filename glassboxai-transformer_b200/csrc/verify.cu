@@ -32,6 +32,7 @@
 // exp2(): ten fp64 instructions where the fp64 pipe is what bounds C.
 #include "gbx_common.cuh"
 #include "kv_cache.cuh"
+#include "row_stats.cuh"
 
 namespace gbx {
 
@@ -92,12 +93,6 @@ __device__ __forceinline__ void vf_push(const double* p, uint32_t rank, double v
 
 // A part of a row: x its maximum, y the sum of 2^((v - x) c2) over it; greedy:
 // x the maximum (NaN where an entry is) and y the bits of its first index.
-__device__ __forceinline__ float2 vf_merge(float2 a, float2 b, float c2)
-{
-    const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.0f : m;
-    return make_float2(m, a.y * vf_exp2((a.x - base) * c2) + b.y * vf_exp2((b.x - base) * c2));
-}
-
 __device__ __forceinline__ float2 vf_better(float2 a, float2 b)
 {
     if (a.x != a.x) return a;
@@ -105,14 +100,14 @@ __device__ __forceinline__ float2 vf_better(float2 a, float2 b)
     return b.x > a.x || (b.x == a.x && __float_as_int(b.y) < __float_as_int(a.y)) ? b : a;
 }
 
-// Of N neighbouring lanes' parts, in a fixed tree.
+// Of N neighbouring lanes' parts, in a fixed tree; the same bits in each of them.
 template <int N>
 __device__ __forceinline__ float2 vf_reduce(float2 v, float c2, int greedy)
 {
 #pragma unroll
     for (int o = 1; o < N; o <<= 1) {
         const float2 w = make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o));
-        v = greedy ? vf_better(v, w) : vf_merge(v, w, c2);
+        v = greedy ? vf_better(v, w) : row_join(v, w, c2, [](float x) { return vf_exp2(x); });
     }
     return v;
 }
@@ -290,10 +285,12 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 2) verify_kernel(const Vf
     }
     __syncthreads();
     vf_wait();   // the other CTAs run
-    // this CTA's part of each row, to every CTA
+    // This CTA's part of each row, to every CTA: one lane's value to all of them,
+    // since each takes part B's decision for itself and they have to agree on it.
     for (int i = tid; i < (nrows * W + 31 & ~31); i += kVfThreads) {
         const int k = i / W, w = i % W;
-        const float2 t = vf_reduce<W>(k < nrows ? s_warp[i] : make_float2(-INFINITY, 0.0f), a.c2, GREEDY);
+        float2 t = vf_reduce<W>(k < nrows ? s_warp[i] : make_float2(-INFINITY, 0.0f), a.c2, GREEDY);
+        t = make_float2(__shfl_sync(0xffffffffu, t.x, 0, W), __shfl_sync(0xffffffffu, t.y, 0, W));
         if (k < nrows)
             for (uint32_t p = w; p < C; p += W) vf_push(s_part + k * C + rank, p, t);
     }
