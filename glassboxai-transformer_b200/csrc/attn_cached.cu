@@ -46,8 +46,8 @@
 // distributed shared memory.  Where that leaves the GPU idle (few heads, a
 // long cache) several clusters share the unit and meet in the workspace.
 //
-// Every wait for a copy is bounded (1 s): a warp that gives up stops its
-// steps, waits (bounded) for the copies it has in flight, and its rows come
+// Every wait for a copy is bounded (1 s): a warp that gives up, as a whole, stops
+// its steps, waits (bounded) for the copies it has in flight, and its rows come
 // out as NaN with GBX_LINEAR_TIMEOUT in the error flag.
 #include <type_traits>
 
@@ -114,6 +114,15 @@ __device__ __forceinline__ void ac_digits(uint32_t w0, uint32_t w1, uint32_t w2,
     d0 = __byte_perm(a, b, 0x5410);
     d1 = __byte_perm(a, b, 0x7632);
     d2 = __byte_perm(__byte_perm(w0, w1, 0x0062), __byte_perm(w2, w3, 0x0062), 0x5410);
+}
+
+// A bounded wait of a whole warp, and one verdict for it.  Every lane polls and
+// reads its own clock and *abort, so some can see the phase complete that others
+// have just given up on; a warp that went two ways from here would wait for good
+// at its next vote or shuffle.
+__device__ __forceinline__ bool ac_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint64_t limit_ns)
+{
+    return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort, limit_ns));
 }
 
 __device__ __forceinline__ uint4 ac_lds(uint32_t at)
@@ -800,7 +809,7 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
     };
     int k = 0;
     for (int step = first; step < steps; step += stride, ++k) {
-        if (limit_ns == 0 || !tc::mbar_wait(bar0 + 8 * slot, phase, abort, limit_ns)) {
+        if (limit_ns == 0 || !ac_wait(bar0 + 8 * slot, phase, abort, limit_ns)) {
             dead = true;
             break;
         }
@@ -821,7 +830,7 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
             ++issued;
         }
         next_slot();
-        if (!tc::mbar_wait(bar0 + 8 * slot, phase, abort, kDeviceWaitNs)) {
+        if (!ac_wait(bar0 + 8 * slot, phase, abort, kDeviceWaitNs)) {
             dead = true;
             break;
         }
@@ -925,7 +934,7 @@ __global__ void __launch_bounds__(32 * (W + 2), HD <= 64 ? 2 : 1) attn_cached_ro
             const int64_t next = copies.look(step + stride);
             for (int which = 0; which < 2; ++which, ++issued) {
                 const int s = issued % NS;
-                if (issued >= NS && !tc::mbar_wait(empty(s), (issued / NS - 1) & 1, abort, kDeviceWaitNs)) goto stop;
+                if (issued >= NS && !ac_wait(empty(s), (issued / NS - 1) & 1, abort, kDeviceWaitNs)) goto stop;
                 copies.issue(which, step, (issued >> 1) & 3, s, full(s), page);
                 __syncwarp();
             }
@@ -958,7 +967,7 @@ __global__ void __launch_bounds__(32 * (W + 2), HD <= 64 ? 2 : 1) attn_cached_ro
             }
         };
         for (int step = first; step < steps; step += stride, ++k) {
-            if (limit_ns == 0 || !tc::mbar_wait(full(slot), phase, abort, limit_ns)) {
+            if (limit_ns == 0 || !ac_wait(full(slot), phase, abort, limit_ns)) {
                 dead = true;
                 break;
             }
@@ -976,7 +985,7 @@ __global__ void __launch_bounds__(32 * (W + 2), HD <= 64 ? 2 : 1) attn_cached_ro
                 else ac_scores<HD, RT>(kb, t0, true, false, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
             }
             leave();
-            if (!tc::mbar_wait(full(slot), phase, abort, kDeviceWaitNs)) {
+            if (!ac_wait(full(slot), phase, abort, kDeviceWaitNs)) {
                 dead = true;
                 break;
             }
