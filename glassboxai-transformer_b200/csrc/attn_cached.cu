@@ -49,6 +49,8 @@
 // Every wait for a copy is bounded (1 s): a warp that gives up, as a whole, stops
 // its steps, waits (bounded) for the copies it has in flight, and its rows come
 // out as NaN with GBX_LINEAR_TIMEOUT in the error flag.
+#include <atomic>
+#include <mutex>
 #include <type_traits>
 
 #include "kv_cache.cuh"
@@ -1046,7 +1048,97 @@ __global__ void __launch_bounds__(256) attn_cached_join_kernel(const AcArgs a, i
 constexpr int kAcWarps = 4, kAcSlots = 3;
 constexpr int kAcRowWarps = 4, kAcRowSlots = 6;
 
-constexpr int kAcSmemPerSM = 228 * 1024;
+// One of the kernels (by head width and 8-row tiles: 1, 2, or 8 for the rows
+// kernel) and the launch that goes with it.
+struct AcKernel {
+    void (*fn)(AcArgs);
+    int threads;
+    size_t smem;
+};
+
+template <int HD, int RT>
+static AcKernel ac_kernel()
+{
+    constexpr bool many = RT == 8;
+    constexpr size_t ring = (size_t)(many ? kAcRowSlots : kAcWarps * kAcSlots) * 4 * ac_pitch(HD);
+    constexpr size_t meet = sizeof(float) * (size_t)((many ? 1 : kAcWarps) + 1) * 8 * RT * (HD + 2);
+    AcKernel k;
+    if constexpr (many) k.fn = attn_cached_rows_kernel<HD, kAcRowWarps, kAcRowSlots>;
+    else k.fn = attn_cached_kernel<HD, RT, kAcWarps, kAcSlots>;
+    k.threads = 32 * (many ? kAcRowWarps + 1 : kAcWarps);
+    k.smem = ring > meet ? ring : meet;
+    return k;
+}
+
+static AcKernel ac_kernel_of(int hd, int rt)
+{
+    auto of = [rt](auto w) {
+        constexpr int HD = decltype(w)::value;
+        return rt == 1 ? ac_kernel<HD, 1>() : rt == 2 ? ac_kernel<HD, 2>() : ac_kernel<HD, 8>();
+    };
+    switch (hd) {
+    case 16: return of(std::integral_constant<int, 16>());
+    case 32: return of(std::integral_constant<int, 32>());
+    case 48: return of(std::integral_constant<int, 48>());
+    case 64: return of(std::integral_constant<int, 64>());
+    case 80: return of(std::integral_constant<int, 80>());
+    case 96: return of(std::integral_constant<int, 96>());
+    case 112: return of(std::integral_constant<int, 112>());
+    default: return of(std::integral_constant<int, 128>());
+    }
+}
+
+static void ac_config(const AcKernel& k, unsigned ctas, int csize, cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr)
+{
+    *cfg = {};
+    cfg->gridDim = dim3(ctas);
+    cfg->blockDim = dim3(k.threads);
+    cfg->dynamicSmemBytes = k.smem;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = (unsigned)csize;
+    attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+    cfg->attrs = attr;
+    cfg->numAttrs = 1;
+}
+
+// How much of a kernel the current device holds at once, asked of the runtime
+// once per kernel and device: what its registers and shared memory allow, and
+// how many clusters of each size its GPCs take.
+struct AcResident {
+    std::atomic<bool> known{false};
+    int ctas;                           // per SM
+    int clusters[kAcMaxCluster + 1];   // on the GPU
+};
+
+static const AcResident* ac_resident(const AcKernel& k, int hd, int rt)
+{
+    constexpr int kDevices = 64;   // as device_info, which has been asked before
+    static AcResident all[kDevices][8][3];
+    static std::mutex lock;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) {
+        set_error(GBX_ECUDA, "gbx_attn_cached: device %d", dev);
+        return nullptr;
+    }
+    AcResident* r = &all[dev][hd / 16 - 1][rt == 8 ? 2 : rt - 1];
+    if (r->known.load(std::memory_order_acquire)) return r;
+    std::lock_guard<std::mutex> hold(lock);
+    if (r->known.load(std::memory_order_relaxed)) return r;
+    bool ok = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) == cudaSuccess &&
+              cudaOccupancyMaxActiveBlocksPerMultiprocessor(&r->ctas, k.fn, k.threads, k.smem) == cudaSuccess && r->ctas > 0;
+    for (int c = 1; ok && c <= kAcMaxCluster; ++c) {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr;
+        ac_config(k, (unsigned)c, c, &cfg, &attr);
+        ok = cudaOccupancyMaxActiveClusters(&r->clusters[c], k.fn, &cfg) == cudaSuccess;
+    }
+    if (!ok) {
+        set_error(GBX_ECUDA, "gbx_attn_cached: occupancy: %s", cudaGetErrorString(cudaGetLastError()));
+        return nullptr;
+    }
+    r->known.store(true, std::memory_order_release);
+    return r;
+}
 
 struct AcPlan {
     int rt, nrb, csize, nsplit;
@@ -1078,24 +1170,21 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bo
     // the workspace, which costs a second launch and is taken where it at least
     // doubles the CTAs.
     const int64_t steps = ((int64_t)max_pages * c->page + kAcTile - 1) / kAcTile;
-    // CTAs resident on an SM.  Registers bound the rows kernel (168 to a thread up to
-    // width 64, 255 beyond) and, with the rings' shared memory, the other (8 rows: 90 at
-    // width 16, 108 up to 64, 147 beyond; 16 rows: 128, 168 and 255).
-    const int64_t by_regs = many ? (c->hd <= 64 ? 2 : 1) : (c->hd <= 16 ? 5 : c->hd <= 64 ? 4 : 3) - (p->rt == 2);
-    const int64_t by_smem = (int64_t)((size_t)kAcSmemPerSM / (kAcWarps * kAcSlots * 4 * ac_pitch(c->hd) + 2048));
-    const int64_t resident = di.sm_count * (many || by_regs < by_smem ? by_regs : by_smem);
+    const AcResident* held = ac_resident(ac_kernel_of(c->hd, p->rt), c->hd, p->rt);
+    if (!held) return GBX_ECUDA;
+    const int64_t resident = (int64_t)di.sm_count * held->ctas;
     int64_t share = resident / p->units;
     if (share > (steps + W - 1) / W) share = (steps + W - 1) / W;
     p->csize = 1;
     p->nsplit = 1;
     while (p->csize < kAcMaxCluster && 2 * p->csize <= share) p->csize *= 2;
     // Rows kernels, which stay on the chip longer, also take the sizes between, where
-    // up to c - 1 CTA places left over in each of the 8 GPCs do not cost a second wave
-    // (64 rows over 3000 tokens: 80 units in threes 36 us against 49 in twos, 42 in sixes
-    // 22.6 against 29.0 in fours; 96 in threes would take 56 against 49).
+    // the GPU holds all the units' clusters at once (64 rows over 3000 tokens: 80 units in
+    // threes 36 us against 49 in twos, 42 in sixes 22.6 against 29.0 in fours; 96 in threes
+    // would take 56 against 49).
     if (many)
         for (int c = kAcMaxCluster - 1; c > p->csize; --c)
-            if (c <= share && p->units * c + 8 * (c - 1) <= resident) {
+            if (c <= share && p->units <= held->clusters[c]) {
                 p->csize = c;
                 break;
             }
@@ -1114,38 +1203,21 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bo
     return GBX_OK;
 }
 
-template <int HD, int RT>
 static int ac_launch(const AcArgs& a, const AcPlan& p, cudaStream_t s)
 {
-    constexpr bool many = RT == 8;
-    constexpr int R = 8 * RT;
-    void (*k)(AcArgs);
-    if constexpr (many) k = attn_cached_rows_kernel<HD, kAcRowWarps, kAcRowSlots>;
-    else k = attn_cached_kernel<HD, RT, kAcWarps, kAcSlots>;
-    const size_t ring = (size_t)(many ? kAcRowSlots : kAcWarps * kAcSlots) * 4 * ac_pitch(HD);
-    const size_t meet = sizeof(float) * (size_t)((many ? 1 : kAcWarps) + 1) * R * (HD + 2);
-    const size_t smem = ring > meet ? ring : meet;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-        return check_launch("gbx_attn_cached: shared-memory attribute");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.units * p.nsplit * p.csize));
-    cfg.blockDim = dim3(32 * (many ? kAcRowWarps + 1 : kAcWarps));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
+    const AcKernel k = ac_kernel_of(a.c.hd, p.rt);
+    cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.csize;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    ac_config(k, (unsigned)(p.units * p.nsplit * p.csize), p.csize, &cfg, attr);
+    cfg.stream = s;
     if (pdl_enabled()) {
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;
     }
-    cudaLaunchKernelEx(&cfg, k, a);
+    cudaLaunchKernelEx(&cfg, k.fn, a);
     if (p.nsplit > 1)
-        launch_row_kernel(attn_cached_join_kernel, dim3((unsigned)p.units), dim3(256), 0, s, a, R);
+        launch_row_kernel(attn_cached_join_kernel, dim3((unsigned)p.units), dim3(256), 0, s, a, 8 * p.rt);
     return check_launch("gbx_attn_cached");
 }
 
@@ -1216,19 +1288,5 @@ extern "C" int gbx_attn_cached(const gbx_kv_cache* cache_host, int layer, const 
     a.vec_out = aligned16(out) && aligned16(out_lo) && ld_out % 4 == 0;
     a.vec = aligned16(q_hi) && aligned16(q_lo) && ld % 4 == 0;
     a.first_wait_ns = first_wait_limit_ns();
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    auto launch = [&](auto hd) {
-        constexpr int HD = decltype(hd)::value;
-        return p.rt == 1 ? ac_launch<HD, 1>(a, p, s) : p.rt == 2 ? ac_launch<HD, 2>(a, p, s) : ac_launch<HD, 8>(a, p, s);
-    };
-    switch (a.c.hd) {
-    case 16: return launch(std::integral_constant<int, 16>());
-    case 32: return launch(std::integral_constant<int, 32>());
-    case 48: return launch(std::integral_constant<int, 48>());
-    case 64: return launch(std::integral_constant<int, 64>());
-    case 80: return launch(std::integral_constant<int, 80>());
-    case 96: return launch(std::integral_constant<int, 96>());
-    case 112: return launch(std::integral_constant<int, 112>());
-    default: return launch(std::integral_constant<int, 128>());
-    }
+    return ac_launch(a, p, reinterpret_cast<cudaStream_t>(stream));
 }
