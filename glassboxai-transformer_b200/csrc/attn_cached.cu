@@ -10,8 +10,9 @@
 // made of 8-bit digits too, three of them (24-bit fixed point):
 //   - a query row, relative to its largest entry: x = sum_k 256^k D_k with
 //     signed digits, D_k . c by mma.sync.m16n8k32.s8.s8, exact;
-//   - a weight, relative to the largest of its row among the step's 64
-//     tokens: unsigned digits, mma.m16n8k32.u8.s8, exact.
+//   - a weight times its page's value scale, relative to the largest such
+//     product of its row among the step's 64 tokens: unsigned digits,
+//     mma.m16n8k32.u8.s8, exact.
 // No code is converted (five instructions per four codes in an f16 form), and
 // no sum inside the tensor cores is rounded.  A tile's 16 rows are 8 query
 // rows: rows 0-7 hold digit 0 and rows 8-15 digit 1 of one instruction, a
@@ -68,6 +69,7 @@ constexpr float kAcQTop = 8355704.0f;
 // A weight is 2^(x - max + 23 - 2^-19): just below 2^23 at most, so that adding 2^23
 // leaves it, rounded, in the low 23 bits of the float.
 constexpr float kAcPOff = 22.99999809265137f;
+constexpr float kAcRoom = 1.00000762939453125f;   // 1 + 2^-17
 
 struct AcArgs {
     KvLayer c;
@@ -349,8 +351,9 @@ __device__ __forceinline__ void ac_queries(const AcArgs& a, const AcUnit& u, int
 // `pitch` bytes apart), the running maximum and sum, and the weights' digits.  ks, vs: the scales of group
 // cc; seen: that group can be read.  edge: some valid
 // row does not see all 64 (rows past the unit's end hold zero queries and are never stored).
+// one: all of them are seen and lie in one page, whose scale is all there is.
 template <int HD, int RT>
-__device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool edge, float ks, float vs,
+__device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool edge, bool one, float ks, float vs,
                                           const AcDigits<RT, ac_chunks(HD)>& q, const float (&qs)[RT], const int (&limit)[RT],
                                           float (&m)[RT], float (&l)[RT], AcDigits<RT, 2>& p, float (&alpha)[RT], float (&beta)[RT],
                                           const AcConst& kc)
@@ -375,16 +378,10 @@ __device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool e
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][g] = d[rt];
     }
-    // the step's largest value scale; a NaN scale stays in the ratio, where
-    // only the rows that see its group meet it
-    float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
-    vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-    const float vr = vmax > 0.0f ? __fdividef(vs, vmax) : (vs == vs ? 0.0f : vs);
-    vmax = vmax > 0.0f ? vmax : 0.0f;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float2 f = splat2(qs[rt] * ks);
-        float mt = -INFINITY;
+        float top = -INFINITY;   // of this lane's group
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
             s[rt][g] = __fmul2_rn(s[rt][g], f);
@@ -393,9 +390,9 @@ __device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool e
                 if (!seen || t >= limit[rt]) s[rt][g].x = -INFINITY;
                 if (!seen || t + 1 >= limit[rt]) s[rt][g].y = -INFINITY;
             }
-            mt = fmaxf(fmaxf(mt, s[rt][g].x), s[rt][g].y);
+            top = fmaxf(fmaxf(top, s[rt][g].x), s[rt][g].y);
         }
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+        float mt = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
         const float mx = fmaxf(m[rt], mt), base = mx == -INFINITY ? 0.0f : mx;
         alpha[rt] = ac_exp2(m[rt] - base);
@@ -404,18 +401,32 @@ __device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool e
         // the maximum is taken off first, exactly where it counts; in one addition with the
         // 23 its rounding would pass 2^-19 from |max| = 32 on (0.3 % of the time)
         const float2 less = splat2(mt == -INFINITY ? 0.0f : -mt), sub = splat2(mt == -INFINITY ? 0.0f : kAcPOff);
-        const float vrr = !edge || t0 + 16 * cc < limit[rt] ? vr : 0.0f;
+        // The digits are relative to the row's largest product of weight and value scale among
+        // the groups it sees, so that large values it does not see, or hardly weighs, cost
+        // the others no bits.  kAcRoom keeps the roundings of the two exponentials and the
+        // quotient below the digits' end.  A group whose weights are all below 2^-126 of the
+        // step's largest counts as none, and so does a step whose products are below 2^-126.
+        // With one scale that product is the scale itself, the largest weight being 1.
+        float most = vs, vr = 1.0f;
+        if (!one) {
+            const float part = ac_exp2(top + less.x) * vs;   // NaN of a NaN scale: not taken by the maximum
+            most = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)) * kAcRoom;
+            most = most >= 1.17549435e-38f ? most : 0.0f;
+            vr = most > 0.0f && part > 0.0f ? __fdividef(vs, most) : 0.0f;
+        }
         float2 sum = make_float2(0.0f, 0.0f), y[8];
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
             float2 x = __fadd2_rn(__fadd2_rn(s[rt][g], less), sub);
             x = make_float2(ac_exp2(x.x), ac_exp2(x.y));
             sum = __fadd2_rn(sum, x);
-            y[g] = __ffma2_rn(x, splat2(vrr), kc.two23);
+            y[g] = one ? __fadd2_rn(x, kc.two23) : __ffma2_rn(x, splat2(vr), kc.two23);
         }
-        // a NaN scale: its digits are no numbers, the sum says so
-        l[rt] = fmaf(l[rt], alpha[rt], fmaf(vrr, 0.0f, sum.x + sum.y) * beta[rt]);
-        beta[rt] *= vmax;
+        // a value scale that is NaN, where the row sees its group: the sum says so
+        const float seen_vs = !edge || t0 + 16 * cc < limit[rt] ? vs : 0.0f;
+        l[rt] = fmaf(l[rt], alpha[rt], fmaf(seen_vs, 0.0f, sum.x + sum.y) * beta[rt]);
+        beta[rt] *= most;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
             ac_digits(__float_as_uint(y[2 * w].x), __float_as_uint(y[2 * w].y), __float_as_uint(y[2 * w + 1].x),
@@ -721,9 +732,15 @@ struct AcCopies {
 };
 
 // HD: head width; RT: 8-row tiles; W: warps; NS: slots of a warp's ring, each
-// the keys or the values of one step.
-template <int HD, int RT, int W, int NS>
-__global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
+// the keys or the values of one step; ONE: pages of 64 tokens or more, so that a
+// step has one value scale.  A kernel for both asks in every step, or forms four
+// groups' products where there is one scale: 2 x 512 rows over 2048 tokens take
+// 60 us in pages of 64 (ONE), 61 when each step asks, 63 by products; 300 rows of
+// 12 heads over 4000 tokens in pages of 16 37 (35 with weights alone as the
+// largest, which loses the bits of pages with smaller values).  16 rows of width
+// 32 are kept to the 128 registers that four CTAs to an SM leave (28 us against 32).
+template <int HD, int RT, int W, int NS, bool ONE>
+__global__ void __launch_bounds__(32 * W, HD == 32 && RT == 2 ? 4 : 0) attn_cached_kernel(const AcArgs a)
 {
     grid_dependency_wait();
     constexpr int R = 8 * RT, T = 32 * W;
@@ -823,8 +840,8 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
         AcDigits<RT, 2> p;
         float alpha[RT], beta[RT];
         const uint32_t kb = ring + slot * slot_bytes;
-        if (edge) ac_scores<HD, RT>(kb, t0, seen, true, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
-        else ac_scores<HD, RT>(kb, t0, true, false, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+        if (edge) ac_scores<HD, RT>(kb, t0, seen, true, false, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+        else ac_scores<HD, RT>(kb, t0, true, false, ONE, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
         // the keys have been read: operation 2k + NS
         __syncwarp();
         if (NS == 3 ? step + stride < steps : step + 2 * stride < steps) {
@@ -876,7 +893,7 @@ __global__ void __launch_bounds__(32 * W) attn_cached_kernel(const AcArgs a)
 // The launch bound is one warp more than there are, which makes the register limit
 // 168: from 169 on an SM's four schedulers take 8 warps, one CTA, instead of 12
 // (width 32: 1038 us with an unbounded kernel's schedule, 970 with this one).
-template <int HD, int W, int NS>
+template <int HD, int W, int NS, bool ONE>
 __global__ void __launch_bounds__(32 * (W + 2), HD <= 64 ? 2 : 1) attn_cached_rows_kernel(const AcArgs a)
 {
     grid_dependency_wait();
@@ -983,8 +1000,8 @@ __global__ void __launch_bounds__(32 * (W + 2), HD <= 64 ? 2 : 1) attn_cached_ro
                 const bool seen = !(ks == 0.0f && signbit(ks));
                 const bool edge = __any_sync(0xffffffffu, !seen) || t0 + kAcTile > wmin;
                 const uint32_t kb = ring + slot * slot_bytes;
-                if (edge) ac_scores<HD, RT>(kb, t0, seen, true, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
-                else ac_scores<HD, RT>(kb, t0, true, false, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+                if (edge) ac_scores<HD, RT>(kb, t0, seen, true, false, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
+                else ac_scores<HD, RT>(kb, t0, true, false, ONE, ks, vs, q, qs, limit, m, l, p, alpha, beta, kc);
             }
             leave();
             if (!ac_wait(full(slot), phase, abort, kDeviceWaitNs)) {
@@ -1048,8 +1065,8 @@ __global__ void __launch_bounds__(256) attn_cached_join_kernel(const AcArgs a, i
 constexpr int kAcWarps = 4, kAcSlots = 3;
 constexpr int kAcRowWarps = 4, kAcRowSlots = 6;
 
-// One of the kernels (by head width and 8-row tiles: 1, 2, or 8 for the rows
-// kernel) and the launch that goes with it.
+// One of the kernels (by head width; 8-row tiles: 1, 2, or 8 for the rows kernel;
+// ONE) and the launch that goes with it.
 struct AcKernel {
     void (*fn)(AcArgs);
     int threads;
@@ -1057,24 +1074,26 @@ struct AcKernel {
 };
 
 template <int HD, int RT>
-static AcKernel ac_kernel()
+static AcKernel ac_kernel(bool one)
 {
     constexpr bool many = RT == 8;
     constexpr size_t ring = (size_t)(many ? kAcRowSlots : kAcWarps * kAcSlots) * 4 * ac_pitch(HD);
     constexpr size_t meet = sizeof(float) * (size_t)((many ? 1 : kAcWarps) + 1) * 8 * RT * (HD + 2);
     AcKernel k;
-    if constexpr (many) k.fn = attn_cached_rows_kernel<HD, kAcRowWarps, kAcRowSlots>;
-    else k.fn = attn_cached_kernel<HD, RT, kAcWarps, kAcSlots>;
+    if constexpr (many)
+        k.fn = one ? attn_cached_rows_kernel<HD, kAcRowWarps, kAcRowSlots, true> : attn_cached_rows_kernel<HD, kAcRowWarps, kAcRowSlots, false>;
+    else
+        k.fn = one ? attn_cached_kernel<HD, RT, kAcWarps, kAcSlots, true> : attn_cached_kernel<HD, RT, kAcWarps, kAcSlots, false>;
     k.threads = 32 * (many ? kAcRowWarps + 1 : kAcWarps);
     k.smem = ring > meet ? ring : meet;
     return k;
 }
 
-static AcKernel ac_kernel_of(int hd, int rt)
+static AcKernel ac_kernel_of(int hd, int rt, bool one)
 {
-    auto of = [rt](auto w) {
+    auto of = [rt, one](auto w) {
         constexpr int HD = decltype(w)::value;
-        return rt == 1 ? ac_kernel<HD, 1>() : rt == 2 ? ac_kernel<HD, 2>() : ac_kernel<HD, 8>();
+        return rt == 1 ? ac_kernel<HD, 1>(one) : rt == 2 ? ac_kernel<HD, 2>(one) : ac_kernel<HD, 8>(one);
     };
     switch (hd) {
     case 16: return of(std::integral_constant<int, 16>());
@@ -1110,17 +1129,17 @@ struct AcResident {
     int clusters[kAcMaxCluster + 1];   // on the GPU
 };
 
-static const AcResident* ac_resident(const AcKernel& k, int hd, int rt)
+static const AcResident* ac_resident(const AcKernel& k, int hd, int rt, bool one)
 {
     constexpr int kDevices = 64;   // as device_info, which has been asked before
-    static AcResident all[kDevices][8][3];
+    static AcResident all[kDevices][8][3][2];
     static std::mutex lock;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) {
         set_error(GBX_ECUDA, "gbx_attn_cached: device %d", dev);
         return nullptr;
     }
-    AcResident* r = &all[dev][hd / 16 - 1][rt == 8 ? 2 : rt - 1];
+    AcResident* r = &all[dev][hd / 16 - 1][rt == 8 ? 2 : rt - 1][one];
     if (r->known.load(std::memory_order_acquire)) return r;
     std::lock_guard<std::mutex> hold(lock);
     if (r->known.load(std::memory_order_relaxed)) return r;
@@ -1142,6 +1161,7 @@ static const AcResident* ac_resident(const AcKernel& k, int hd, int rt)
 
 struct AcPlan {
     int rt, nrb, csize, nsplit;
+    bool one;   // a step's tokens lie in one page
     int64_t units, ws_floats;
 };
 
@@ -1157,6 +1177,7 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bo
     // split the warps, going through the steps together (4 x 20 rows of 4 query heads
     // to a key head of width 128 over 2000 tokens: 24 us against 32 in blocks of 16)
     p->rt = rows <= 8 ? 1 : rows <= 16 ? 2 : 8;
+    p->one = c->page >= kAcTile;
     const bool many = p->rt == 8;
     const int R = 8 * p->rt, W = many ? 1 : kAcWarps;   // warps that split the steps
     const int64_t nrb = (rows + R - 1) / R;
@@ -1170,7 +1191,7 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bo
     // the workspace, which costs a second launch and is taken where it at least
     // doubles the CTAs.
     const int64_t steps = ((int64_t)max_pages * c->page + kAcTile - 1) / kAcTile;
-    const AcResident* held = ac_resident(ac_kernel_of(c->hd, p->rt), c->hd, p->rt);
+    const AcResident* held = ac_resident(ac_kernel_of(c->hd, p->rt, p->one), c->hd, p->rt, p->one);
     if (!held) return GBX_ECUDA;
     const int64_t resident = (int64_t)di.sm_count * held->ctas;
     int64_t share = resident / p->units;
@@ -1205,7 +1226,7 @@ static int ac_plan(const gbx_kv_cache* c, int B, int S, int H, int max_pages, bo
 
 static int ac_launch(const AcArgs& a, const AcPlan& p, cudaStream_t s)
 {
-    const AcKernel k = ac_kernel_of(a.c.hd, p.rt);
+    const AcKernel k = ac_kernel_of(a.c.hd, p.rt, p.one);
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
     ac_config(k, (unsigned)(p.units * p.nsplit * p.csize), p.csize, &cfg, attr);

@@ -547,12 +547,13 @@ int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* src, const 
  * out_lo its tf32 pair, the x operand of the output projection.  S = 1 is a
  * decode step, a few rows score drafted tokens, many are the next chunk of a
  * prompt.  The codes enter the tensor cores exactly; a query row is 24-bit
- * fixed point relative to its largest entry, a weight relative to the
- * largest weight of its row among 64 neighbouring tokens; sums inside those
- * are exact, all others fp32.  The result is that of fp32 attention over the
- * cached values to within rounding.  A page read by a valid row whose scale
- * is NaN gives NaN; a row that sees no page that can be read gives 0.  out
- * and out_lo must overlap neither each other nor q.
+ * fixed point relative to its largest entry, a weight times its page's value
+ * scale 23-bit relative to the largest such product that its row sees among 64
+ * neighbouring tokens; sums inside those are exact, all others fp32.  The
+ * result is that of fp32 attention over the cached values to within rounding.
+ * A page read by a valid row whose scale is NaN gives NaN; a row that sees no
+ * page that can be read gives 0.  out and out_lo must overlap neither each
+ * other nor q.
  *
  * workspace: device floats, at least gbx_attn_cached_workspace(...) of them
  * (0: none needed, NULL will do); long caches read by few heads are cut into
