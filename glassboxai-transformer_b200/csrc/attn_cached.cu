@@ -69,6 +69,11 @@ constexpr float kAcQTop = 8355704.0f;
 // A weight is 2^(x - max + 23 - 2^-19): just below 2^23 at most, so that adding 2^23
 // leaves it, rounded, in the low 23 bits of the float.
 constexpr float kAcPOff = 22.99999809265137f;
+// A row's sums of digits and codes reach 2^23 times the values' own; held with this
+// factor they stay finite for values up to 2^118 in size, and lose nothing of the
+// smallest scale there is (2^-107).  The scales are read with it, and the weights'
+// sum gets it after the last step, so that it leaves with the quotient.
+constexpr float kAcDown = 1.9073486328125e-6f;    // 2^-19
 constexpr float kAcRoom = 1.00000762939453125f;   // 1 + 2^-17
 
 struct AcArgs {
@@ -361,6 +366,7 @@ __device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool e
     const int lane = threadIdx.x & 31, n = lane >> 2, cc = lane & 3;
     constexpr int NCH = ac_chunks(HD) / 2, pitch = ac_pitch(HD);
     float2 s[RT][8];
+    vs *= kAcDown;
     // key side: this lane's tokens are 2g + (n & 1) of group n / 2
     // columns past the head's last 16 (their query digits are 0) are read from
     // those: 16 bytes further, a slot's last token would leave the ring
@@ -405,7 +411,7 @@ __device__ __forceinline__ void ac_scores(uint32_t kb, int t0, bool seen, bool e
         // the groups it sees, so that large values it does not see, or hardly weighs, cost
         // the others no bits.  kAcRoom keeps the roundings of the two exponentials and the
         // quotient below the digits' end.  A group whose weights are all below 2^-126 of the
-        // step's largest counts as none, and so does a step whose products are below 2^-126.
+        // step's largest counts as none, and so does a step whose products are below 2^-107.
         // With one scale that product is the scale itself, the largest weight being 1.
         float most = vs, vr = 1.0f;
         if (!one) {
@@ -864,6 +870,8 @@ __global__ void __launch_bounds__(32 * W, HD == 32 && RT == 2 ? 4 : 0) attn_cach
         pg[1] = pg[2];
         pg[2] = look(step + 3 * stride);
     }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) l[rt] *= kAcDown;
     if (dead) {
         // the copies in flight land before anything else happens to this memory
         *abort = 1;
@@ -1011,6 +1019,8 @@ __global__ void __launch_bounds__(32 * (W + 2), HD <= 64 ? 2 : 1) attn_cached_ro
             if (some) ac_values<HD, RT>(ring + slot * slot_bytes, p, alpha, beta, o, kc);
             leave();
         }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) l[rt] *= kAcDown;
         if (dead) {
             *abort = 1;
             if (lane == 0) kv_flag(c.err, GBX_LINEAR_TIMEOUT);

@@ -550,7 +550,8 @@ int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* src, const 
  * fixed point relative to its largest entry, a weight times its page's value
  * scale 23-bit relative to the largest such product that its row sees among 64
  * neighbouring tokens; sums inside those are exact, all others fp32.  The
- * result is that of fp32 attention over the cached values to within rounding.
+ * result is that of fp32 attention over the cached values (up to 2^118 in
+ * size) to within rounding.
  * A page read by a valid row whose scale is NaN gives NaN; a row that sees no
  * page that can be read gives 0.  out and out_lo must overlap neither each
  * other nor q.

@@ -102,3 +102,16 @@ def test_pages_of_zero_and_of_tiny_values(gbx, cuda, S):
         s.upload()
         q = s.rng.standard_normal((1, S, heads, hd)).astype(np.float32)
         check(s, q, [L], [S], 8.0)
+
+
+@pytest.mark.parametrize("S,hd,G", SHAPES)
+@pytest.mark.parametrize("P", [16, 64])
+def test_large_values(gbx, cuda, S, hd, G, P):
+    """Values up to 1e35: their sums in fixed point, 2^36 units and more, stay finite too."""
+    heads, L = 2, 200 + S
+    s = Setup(gbx, P, heads, hd, 1, L, seed=S * hd + 1)
+    s.ref.scale[1][:] = np.float32(1e35 / 127) * s.rng.uniform(0.3, 1, s.ref.scale[1].shape).astype(np.float32)
+    s.ref.codes[1][:] = 127 - np.abs(s.ref.codes[1]) // 2
+    s.upload()
+    q = s.rng.standard_normal((1, S, heads * G, hd)).astype(np.float32) * 0.1
+    check(s, q, [L], [S], np.sqrt(hd))
