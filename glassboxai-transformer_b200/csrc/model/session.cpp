@@ -17,7 +17,9 @@
 namespace gbx {
 
 // ---------------------------------------------------------------- pages
-PageTable::PageTable(int64_t pages, int pageSize) : pageSize_(pageSize), refs_((size_t)(pages < 0 ? 0 : pages), 0)
+// (pages of no tokens: none)
+PageTable::PageTable(int64_t pages, int pageSize)
+    : pageSize_(pageSize < 1 ? 1 : pageSize), refs_((size_t)(pages < 0 || pageSize < 1 ? 0 : pages), 0)
 {
     free_.resize(refs_.size());
     for (size_t i = 0; i < free_.size(); ++i) free_[i] = (int32_t)i;   // sorted: a heap already
