@@ -273,10 +273,6 @@ bool Session::check(const std::vector<int>& seqs, const std::vector<int>& ids, c
 {
     err_.clear();
     if (!ok_) return fail("session: not open");
-    const gbx_kv_cache& c = impl_->cache;
-    if (!model_.isModelLoaded() || model_.getNumLayers() != c.layers || model_.getNumHeads() != c.heads ||
-        model_.getEmbedDim() != c.heads * c.hd)
-        return fail("session: the model is not the one it was opened on");
     if (seqs.empty() || seqs.size() != counts.size()) return fail("session: a count for each of at least one sequence");
     int64_t all = 0;
     *S = 0;

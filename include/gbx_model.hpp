@@ -265,7 +265,8 @@ private:
 // prefix.  Keys and values are held in 8 bits (see gbx_kv_append), so logits
 // differ from forward's by that rounding; a prompt that starts its sequences
 // attends over its unrounded keys and values.  The model must outlive the
-// session and not be loaded again meanwhile; a session is used by one thread at a time, as the model is.
+// session (a model is loaded once: a second loadModel fails and changes nothing).
+// A session is used by one thread at a time, as the model is.
 class Session {
 public:
     Session(TransformerModel& model, int64_t pages, int pageSize = 64);

@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+from gguf_writer import GGML_F32, write_tiny_gpt2
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "glassboxai-transformer_b200")
 
@@ -25,3 +27,9 @@ def run(*args):
 
 def test_page_sizes_that_cannot_be(session_check):
     run(session_check, "sizes")
+
+@pytest.mark.gpu
+def test_a_model_is_loaded_once(session_check, cuda, tmp_path):
+    path = str(tmp_path / "m.gguf")
+    write_tiny_gpt2(path, GGML_F32, d=128, heads=2, ff=256, layers=2, ctx=64, vocab=700, seed=1)
+    run(session_check, "reload", path)
