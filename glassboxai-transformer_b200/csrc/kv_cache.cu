@@ -426,37 +426,38 @@ struct KvPool {
 
 // One CTA per (pair, layer, K or V) and, where those are fewer than four to an
 // SM, part of the page: 600 pages of 24 layers in 287 us, 6.6 TB/s, two pages of 5 in
-// 2.8 (8.2 whole).  A page of a layer is one contiguous run of bytes.  Before it stores, the CTA looks its target up among all
-// sources and earlier targets (n words each, from L2): a pair that would race
-// with another is left out, by every CTA alike.
+// 2.8 (8.2 whole).  A page of a layer is one contiguous run of bytes.  Before it stores, the CTA looks its target up among
+// the earlier targets and, where pages move within one pool, all sources (n words each, from L2):
+// a pair that would race with another is left out, by every CTA alike.
 __global__ void __launch_bounds__(256)
-kv_copy_kernel(const KvPool c, const int32_t* src, const int32_t* dst, int n)
+kv_copy_kernel(const KvPool c, const KvPool t, const int32_t* src, const int32_t* dst, int n)
 {
     grid_dependency_wait();
+    const bool within = c.k == t.k;
     const int i = blockIdx.x, layer = blockIdx.y >> 1, which = blockIdx.y & 1;
     const int from = src[i], to = dst[i];
     const bool first = blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0;
-    if ((uint64_t)(int64_t)from >= (uint64_t)c.pages || (uint64_t)(int64_t)to >= (uint64_t)c.pages) {
+    if ((uint64_t)(int64_t)from >= (uint64_t)c.pages || (uint64_t)(int64_t)to >= (uint64_t)t.pages) {
         if (first) kv_flag(c.err, GBX_KV_BAD_PAGE);
         return;
     }
-    if (from == to) return;
+    if (within && from == to) return;
     bool clash = false;
-    for (int j = threadIdx.x; j < n; j += 256) clash |= (src[j] == to) | (j < i && dst[j] == to);
+    for (int j = threadIdx.x; j < n; j += 256) clash |= (within && src[j] == to) | (j < i && dst[j] == to);
     if (__syncthreads_or(clash)) {
         if (first) kv_flag(c.err, GBX_KV_BAD_PAIR);
         return;
     }
-    int8_t* base = (which ? c.v : c.k) + (int64_t)layer * c.pages * c.page_bytes;
-    const uint4* s = reinterpret_cast<const uint4*>(base + from * c.page_bytes);
-    uint4* d = reinterpret_cast<uint4*>(base + to * c.page_bytes);
+    const uint4* s = reinterpret_cast<const uint4*>((which ? c.v : c.k) + ((int64_t)layer * c.pages + from) * c.page_bytes);
+    uint4* d = reinterpret_cast<uint4*>((which ? t.v : t.k) + ((int64_t)layer * t.pages + to) * c.page_bytes);
     const int words = (int)(c.page_bytes >> 4), part = (words + (int)gridDim.z - 1) / (int)gridDim.z;
     const int end = min(words, ((int)blockIdx.z + 1) * part);
 #pragma unroll 4
     for (int e = (int)blockIdx.z * part + threadIdx.x; e < end; e += 256) d[e] = s[e];
     if (blockIdx.z) return;
-    float* sc = (which ? c.vs : c.ks) + (int64_t)layer * c.pages * c.heads;
-    for (int e = threadIdx.x; e < c.heads; e += 256) sc[(int64_t)to * c.heads + e] = sc[(int64_t)from * c.heads + e];
+    const float* ss = (which ? c.vs : c.ks) + ((int64_t)layer * c.pages + from) * c.heads;
+    float* ds = (which ? t.vs : t.ks) + ((int64_t)layer * t.pages + to) * c.heads;
+    for (int e = threadIdx.x; e < c.heads; e += 256) ds[e] = ss[e];
 }
 
 // ---------------------------------------------------------------- host checks
@@ -589,14 +590,10 @@ extern "C" int gbx_kv_read(const gbx_kv_cache* cache_host, int layer, const int3
     return check_launch("gbx_kv_read");
 }
 
-extern "C" int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* src, const int32_t* dst, int n,
-                                 int* err_flag, gbx_stream_t stream)
+namespace gbx {
+
+static KvPool kv_pool(const gbx_kv_cache& h, int* err)
 {
-    if (int rc = kv_check_cache(cache_host, "gbx_kv_copy_pages")) return rc;
-    if (n < 0) return set_error(GBX_EINVAL, "gbx_kv_copy_pages: n=%d", n);
-    if (n == 0) return GBX_OK;
-    if (!src || !dst) return set_error(GBX_EINVAL, "gbx_kv_copy_pages: null pointer");
-    const gbx_kv_cache& h = *cache_host;
     KvPool c;
     c.k = h.k;
     c.v = h.v;
@@ -606,14 +603,33 @@ extern "C" int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* 
     c.pages = h.pages;
     c.heads = h.heads;
     c.layers = h.layers;
-    c.err = err_flag;
+    c.err = err;
+    return c;
+}
+
+int kv_copy_across(const gbx_kv_cache* from, const gbx_kv_cache* to, const int32_t* src, const int32_t* dst, int n, int* err_flag,
+                   gbx_stream_t stream)
+{
+    const KvPool c = kv_pool(*from, err_flag);
     DeviceInfo di;
     if (device_info(&di) != GBX_OK) return GBX_ECUDA;
-    int64_t parts = 4 * (int64_t)di.sm_count / ((int64_t)n * h.layers * 2), most = c.page_bytes / 4096;   // 256 x 16 bytes
+    int64_t parts = 4 * (int64_t)di.sm_count / ((int64_t)n * c.layers * 2), most = c.page_bytes / 4096;   // 256 x 16 bytes
     if (parts > most) parts = most;
     if (parts < 1) parts = 1;
     if (parts > 65535) parts = 65535;
-    launch_row_kernel(kv_copy_kernel, dim3((unsigned)n, (unsigned)h.layers * 2, (unsigned)parts), dim3(256), 0,
-                      reinterpret_cast<cudaStream_t>(stream), c, src, dst, n);
+    launch_row_kernel(kv_copy_kernel, dim3((unsigned)n, (unsigned)c.layers * 2, (unsigned)parts), dim3(256), 0,
+                      reinterpret_cast<cudaStream_t>(stream), c, kv_pool(*to, err_flag), src, dst, n);
     return check_launch("gbx_kv_copy_pages");
+}
+
+}  // namespace gbx
+
+extern "C" int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* src, const int32_t* dst, int n,
+                                 int* err_flag, gbx_stream_t stream)
+{
+    if (int rc = kv_check_cache(cache_host, "gbx_kv_copy_pages")) return rc;
+    if (n < 0) return set_error(GBX_EINVAL, "gbx_kv_copy_pages: n=%d", n);
+    if (n == 0) return GBX_OK;
+    if (!src || !dst) return set_error(GBX_EINVAL, "gbx_kv_copy_pages: null pointer");
+    return kv_copy_across(cache_host, cache_host, src, dst, n, err_flag, stream);
 }

@@ -57,4 +57,9 @@ int kv_check_cache(const gbx_kv_cache* c, const char* what);
 int kv_layer(const gbx_kv_cache* c, int layer, const int32_t* table, int max_pages, const int32_t* kv_len,
              const int32_t* n_new, int B, int S, int* err, const char* what, KvLayer* out);
 
+// Page src[i] of one pool becomes page dst[i] of another of the same layers, heads,
+// page and hd (or of the same pool, as gbx_kv_copy_pages), in every layer.
+int kv_copy_across(const gbx_kv_cache* from, const gbx_kv_cache* to, const int32_t* src, const int32_t* dst, int n, int* err,
+                   gbx_stream_t stream);
+
 }  // namespace gbx

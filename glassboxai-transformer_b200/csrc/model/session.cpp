@@ -16,6 +16,10 @@
 
 namespace gbx {
 
+// kv_cache.cu: pages src of one pool become pages dst of another
+int kv_copy_across(const gbx_kv_cache* from, const gbx_kv_cache* to, const int32_t* src, const int32_t* dst, int n, int* err,
+                   gbx_stream_t stream);
+
 // ---------------------------------------------------------------- pages
 // (pages of no tokens: none)
 PageTable::PageTable(int64_t pages, int pageSize)
@@ -186,20 +190,6 @@ struct OnDevice {   // the model's device current, for a scope
     }
 };
 
-// Puts a page table back as it was unless the call came to its end: the pages a
-// step copied from, or would have written behind the sequences' ends, are
-// still theirs.
-struct Restore {
-    PageTable& table;
-    PageTable saved;
-    bool done = false;
-    explicit Restore(PageTable& t) : table(t), saved(t) {}
-    ~Restore()
-    {
-        if (!done) table = std::move(saved);
-    }
-};
-
 }  // namespace
 
 struct Session::Impl {
@@ -209,14 +199,60 @@ struct Session::Impl {
     Array ws;                // of gbx_attn_cached
     Array select;            // of token selection and verification
     Array pairs;             // of page copies
+    // What a step's appends can change of the tokens before it: a sequence's last
+    // page, where it is not full, has its scales raised and its codes rounded anew
+    // (or, by a NaN, lost).  Such pages are copied here first.
+    gbx_kv_cache saved = {};
+    Array sk, sv, sks, svs;
+    std::vector<int32_t> savedPages;           // page of the pool that saved page i is a copy of
+    const int32_t* savedIds = nullptr;         // the same on the device, and after them 0, 1, ..
     int32_t* err = nullptr;
     int device = -1;
     cudaStream_t stream = nullptr;   // the model's
     ~Impl()
     {
         OnDevice on(device);
-        for (Array* a : {&k, &v, &ks, &vs, &step, &ws, &select, &pairs}) a->release();
+        for (Array* a : {&k, &v, &ks, &vs, &step, &ws, &select, &pairs, &sk, &sv, &sks, &svs}) a->release();
         if (err) cudaFree(err);
+    }
+    // Room for n pages beside the pool.
+    bool ensureSaved(size_t n)
+    {
+        const size_t scales = (size_t)cache.layers * n * cache.heads, codes = scales * cache.page * cache.hd;
+        if (!sk.ensure(codes) || !sv.ensure(codes) || !sks.ensure(scales * 4) || !svs.ensure(scales * 4)) return false;
+        saved = cache;
+        saved.k = (int8_t*)sk.p;
+        saved.v = (int8_t*)sv.p;
+        saved.k_scale = (float*)sks.p;
+        saved.v_scale = (float*)svs.p;
+        saved.pages = (int64_t)n;
+        return true;
+    }
+    // The saved pages' contents back in the pool.
+    bool putBack()
+    {
+        if (savedPages.empty()) return true;
+        OnDevice on(device);
+        const int n = (int)savedPages.size();
+        savedPages.clear();
+        return kv_copy_across(&saved, &cache, savedIds + n, savedIds, n, nullptr, reinterpret_cast<gbx_stream_t>(stream)) == GBX_OK &&
+               cudaStreamSynchronize(stream) == cudaSuccess;
+    }
+};
+
+// Undoes a step that does not come to its end: the pages that it wrote to have
+// their contents back, and the page table is as it was, so that pages it copied
+// from, or took, are again whose they were.
+struct Session::Undo {
+    Session& s;
+    PageTable before;
+    bool done = false;
+    explicit Undo(Session& session) : s(session), before(session.table_) { s.impl_->savedPages.clear(); }
+    ~Undo()
+    {
+        if (done) return;
+        if (!s.impl_->putBack()) s.ok_ = false;   // the sequences' last pages are lost: none of them can be used
+        s.table_ = std::move(before);
     }
 };
 
@@ -294,8 +330,8 @@ bool Session::check(const std::vector<int>& seqs, const std::vector<int>& ids, c
     return true;
 }
 
-// Appends and runs the model; the logits stay in the model's buffer.  The caller
-// puts the page table back if this, or what it does with the logits, fails.
+// Appends and runs the model; the logits stay in the model's buffer.  The caller's
+// Undo takes it back if this, or what it does with the logits, fails.
 bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, bool allRows,
                    const std::vector<int>& padded, int S)
 {
@@ -315,8 +351,18 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
     const int B = (int)seqs.size();
     size_t most = 1;
     for (int s : seqs) most = std::max(most, table_.pagesOf(s).size());
-    // one array: table, lengths, counts, positions
+    // the pages that hold tokens of before and get new ones (each one sequence's own by now)
+    std::vector<int32_t> partial;
+    for (int b = 0; b < B; ++b)
+        if (before[b] % table_.pageSize()) partial.push_back(table_.pagesOf(seqs[b])[(size_t)(before[b] / table_.pageSize())]);
+    // one array: table, lengths, counts, positions, the pairs of page copies, the partial pages and 0, 1, ..
+    const size_t nCopies = copies.src.size(), nPartial = partial.size();
     std::vector<int32_t> host((size_t)B * most + 2 * (size_t)B + (size_t)B * S, 0);
+    const size_t atCopies = host.size(), atPartial = atCopies + 2 * nCopies;
+    host.insert(host.end(), copies.src.begin(), copies.src.end());
+    host.insert(host.end(), copies.dst.begin(), copies.dst.end());
+    host.insert(host.end(), partial.begin(), partial.end());
+    for (size_t i = 0; i < nPartial; ++i) host.push_back((int32_t)i);
     int32_t *kvLen = host.data() + (size_t)B * most, *nNew = kvLen + B, *pos = nNew + B;
     for (int b = 0; b < B; ++b) {
         const std::vector<int32_t>& pages = table_.pagesOf(seqs[b]);
@@ -326,23 +372,25 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
         for (int j = 0; j < counts[b]; ++j) pos[(size_t)b * S + j] = (int32_t)(before[b] + j);
     }
     const int64_t wsFloats = gbx_attn_cached_workspace(&m.cache, B, S, m.cache.heads, (int)most);
+    const gbx_stream_t gs = reinterpret_cast<gbx_stream_t>(m.stream);
     bool good = wsFloats >= 0 && m.step.ensure(host.size() * 4) && m.ws.ensure((size_t)wsFloats * 4 + 4) &&
+                (!nPartial || m.ensureSaved(nPartial)) &&
                 cudaMemcpyAsync(m.step.p, host.data(), host.size() * 4, cudaMemcpyHostToDevice, m.stream) == cudaSuccess;
-    if (good && !copies.src.empty()) {
-        const size_t n = copies.src.size();
-        good = m.pairs.ensure(n * 8) && cudaMemsetAsync(m.err, 0, 4, m.stream) == cudaSuccess &&
-               cudaMemcpyAsync(m.pairs.p, copies.src.data(), n * 4, cudaMemcpyHostToDevice, m.stream) == cudaSuccess &&
-               cudaMemcpyAsync((int32_t*)m.pairs.p + n, copies.dst.data(), n * 4, cudaMemcpyHostToDevice, m.stream) == cudaSuccess &&
-               gbx_kv_copy_pages(&m.cache, (int32_t*)m.pairs.p, (int32_t*)m.pairs.p + n, (int)n, m.err,
-                                 reinterpret_cast<gbx_stream_t>(m.stream)) == GBX_OK;
-    }
+    const int32_t* ints = (const int32_t*)m.step.p;
+    // (the page table makes no pair that clashes or leaves the pool: nothing to report)
+    if (good && nCopies)
+        good = gbx_kv_copy_pages(&m.cache, ints + atCopies, ints + atCopies + nCopies, (int)nCopies, nullptr, gs) == GBX_OK;
+    if (good && nPartial)
+        good = kv_copy_across(&m.cache, &m.saved, ints + atPartial, ints + atPartial + nPartial, (int)nPartial, nullptr, gs) == GBX_OK;
     if (!good) {
         cudaStreamSynchronize(m.stream);
         return fail(std::string("session: preparing the step failed: ") + gbx_last_error());
     }
+    m.savedIds = ints + atPartial;
+    m.savedPages = std::move(partial);
     TransformerModel::CachedStep st;
     st.cache = &m.cache;
-    st.table = (int32_t*)m.step.p;
+    st.table = ints;
     st.maxPages = (int)most;
     st.kvLen = st.table + (size_t)B * most;
     st.nNew = st.kvLen + B;
@@ -363,7 +411,7 @@ std::vector<float> Session::forward(const std::vector<int>& seqs, const std::vec
     std::vector<int> padded;
     std::vector<float> out;
     if (!check(seqs, ids, counts, &S, &padded)) return out;
-    Restore table(table_);
+    Undo undo(*this);
     if (!step(seqs, ids, counts, allRows, padded, S)) return out;
     OnDevice on(impl_->device);
     const size_t V = (size_t)model_.getVocabSize();
@@ -384,7 +432,7 @@ std::vector<float> Session::forward(const std::vector<int>& seqs, const std::vec
         fail("session: device-to-host copy of the logits failed");
         out.clear();
     }
-    table.done = good;
+    undo.done = good;
     return out;
 }
 
@@ -406,7 +454,7 @@ std::vector<int> Session::nextTokens(const std::vector<int>& seqs, const std::ve
         fail("session: cudaMalloc failed");
         return out;
     }
-    Restore table(table_);
+    Undo undo(*this);
     if (!step(seqs, ids, counts, false, padded, S)) return out;
     double* du = (double*)m.select.p;
     int32_t* dids = (int32_t*)(du + B);
@@ -420,7 +468,7 @@ std::vector<int> Session::nextTokens(const std::vector<int>& seqs, const std::ve
         return out;
     }
     out.assign(got.begin(), got.end());
-    table.done = true;
+    undo.done = true;
     return out;
 }
 
@@ -467,7 +515,7 @@ bool Session::verify(const std::vector<int>& seqs, const std::vector<int>& ids, 
     const size_t offLogits = du.size() * 8, offIds = offLogits + logitBytes, offLens = offIds + cut.size() * 4,
                  offOut = offLens + B * 4, offAcc = offOut + B * (size_t)S * 4;
     if (!m.select.ensure(offAcc + B * 4)) return fail("session: cudaMalloc failed");
-    Restore table(table_);
+    Undo undo(*this);
     std::vector<int64_t> before;
     for (int s : seqs) before.push_back(table_.length(s));
     if (!step(seqs, given, counts, true, padded, S)) return false;
@@ -497,7 +545,7 @@ bool Session::verify(const std::vector<int>& seqs, const std::vector<int>& ids, 
         for (int j = 0; j < S; ++j) (*outIds)[b * n1 + j] = out[b * S + j];
         table_.truncate(seqs[b], before[b] + 1 + acc[b]);
     }
-    table.done = true;
+    undo.done = true;
     return true;
 }
 

@@ -96,8 +96,9 @@ int64_t gbx_session_length(gbx_session* s, int seq);
 int64_t gbx_session_free_pages(gbx_session* s);
 /* Appends counts[i] tokens to sequence seqs[i] (ids: n_ids of them, one sequence
  * after another); logits_host receives vocab floats for each sequence's last
- * token, or with all_rows != 0 for every token.  On failure every sequence
- * keeps the length it had. */
+ * token, or with all_rows != 0 for every token.  On failure every sequence is
+ * as it was: its length, and what its pages hold.  (Should the GPU itself have
+ * failed, so that they cannot be put back, the session refuses every later call.) */
 int gbx_session_forward(gbx_session* s, const int32_t* seqs_host, int n_seq, const int32_t* ids_host, int64_t n_ids,
                         const int32_t* counts_host, int all_rows, float* logits_host);
 /* The same, and each sequence's next token (gbx_select_tokens) with the draws

@@ -288,7 +288,8 @@ public:
     // Appends counts[i] tokens to sequence seqs[i] (ids: all of them, one
     // sequence after another) and returns logits: each sequence's last token's,
     // or with allRows every token's, vocab floats each, in the order of ids.
-    // Empty on failure (lastError()), with every sequence at the length it had.
+    // Empty on failure (lastError()), with every sequence as it was: its length, and
+    // what its pages hold.
     std::vector<float> forward(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts,
                                bool allRows = false);
     // forward, and each sequence's next token by the reference's rule
@@ -310,6 +311,7 @@ public:
 
 private:
     struct Impl;
+    struct Undo;
     bool fail(const std::string& msg);
     bool step(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, bool allRows,
               const std::vector<int>& padded, int S);
