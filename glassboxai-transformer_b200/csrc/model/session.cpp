@@ -199,6 +199,7 @@ struct Session::Impl {
     Array ws;                // of gbx_attn_cached
     Array select;            // of token selection and verification
     Array pairs;             // of page copies
+    Array rows;              // a verification's QKV rows of every layer, as tf32 pairs
     // What a step's appends can change of the tokens before it: a sequence's last
     // page, where it is not full, has its scales raised and its codes rounded anew
     // (or, by a NaN, lost).  Such pages are copied here first.
@@ -212,7 +213,7 @@ struct Session::Impl {
     ~Impl()
     {
         OnDevice on(device);
-        for (Array* a : {&k, &v, &ks, &vs, &step, &ws, &select, &pairs, &sk, &sv, &sks, &svs}) a->release();
+        for (Array* a : {&k, &v, &ks, &vs, &step, &ws, &select, &pairs, &rows, &sk, &sv, &sks, &svs}) a->release();
         if (err) cudaFree(err);
     }
     // Room for n pages beside the pool.
@@ -331,12 +332,15 @@ bool Session::check(const std::vector<int>& seqs, const std::vector<int>& ids, c
 }
 
 // Appends and runs the model; the logits stay in the model's buffer.  The caller's
-// Undo takes it back if this, or what it does with the logits, fails.
+// Undo takes it back if this, or what it does with the logits, fails.  keepRows:
+// the layers' QKV rows stay, for keepOnly.
 bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, bool allRows,
-                   const std::vector<int>& padded, int S)
+                   const std::vector<int>& padded, int S, bool keepRows)
 {
     Impl& m = *impl_;
     OnDevice on(m.device);
+    const size_t rowFloats = keepRows ? padded.size() * 3 * (size_t)model_.getEmbedDim() * m.cache.layers : 0;
+    if (!m.rows.ensure(rowFloats * 8)) return fail("session: cudaMalloc of the step's rows failed");
     std::vector<int64_t> before;
     bool even = true, empty = true;
     for (size_t i = 0; i < seqs.size(); ++i) {
@@ -401,7 +405,59 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
     st.even = even;
     st.fresh = even && empty;
     st.allRows = allRows;
+    st.rows = keepRows ? (float*)m.rows.p : nullptr;
+    st.rowsLo = st.rows + rowFloats;
     return model_.runForward(padded, B, nullptr, &st) || fail(model_.lastError());
+}
+
+// Leaves in the cache what a step of keep[b] tokens of sequence b would have: the
+// last step's rejected tokens have raised scales and rounded kept tokens by them.
+// The pages of the sequences with fewer tokens than counts[b] start again from
+// what they held before that step, and the kept rows are appended to them.
+bool Session::keepOnly(const std::vector<int>& seqs, const std::vector<int64_t>& before, const std::vector<int>& counts,
+                       const std::vector<int>& keep, int S)
+{
+    Impl& m = *impl_;
+    const int B = (int)seqs.size(), d = model_.getEmbedDim();
+    // page and place among the saved ones of those to start again, then lengths and counts
+    std::vector<int32_t> pages, places, lens(B), news(B, 0);
+    size_t most = 1;
+    int saved = 0;
+    bool any = false;
+    for (int b = 0; b < B; ++b) {
+        const std::vector<int32_t>& p = table_.pagesOf(seqs[b]);
+        most = std::max(most, p.size());
+        const bool partial = before[b] % table_.pageSize() != 0, fewer = keep[b] < counts[b];
+        if (partial && fewer) {
+            pages.push_back(m.savedPages[saved]);
+            places.push_back(saved);
+        }
+        saved += partial;
+        lens[b] = (int32_t)(before[b] + keep[b]);
+        if (fewer) news[b] = keep[b];
+        any = any || fewer;
+    }
+    if (!any) return true;
+    const size_t n = pages.size();
+    std::vector<int32_t> host(pages);
+    host.insert(host.end(), places.begin(), places.end());
+    host.insert(host.end(), lens.begin(), lens.end());
+    host.insert(host.end(), news.begin(), news.end());
+    const gbx_stream_t gs = reinterpret_cast<gbx_stream_t>(m.stream);
+    int32_t bits = 0;
+    bool good = m.pairs.ensure(host.size() * 4) &&
+                cudaMemcpyAsync(m.pairs.p, host.data(), host.size() * 4, cudaMemcpyHostToDevice, m.stream) == cudaSuccess &&
+                cudaMemsetAsync(m.err, 0, 4, m.stream) == cudaSuccess;
+    const int32_t* ints = (const int32_t*)m.pairs.p;
+    if (good && n) good = kv_copy_across(&m.saved, &m.cache, ints + n, ints, (int)n, m.err, gs) == GBX_OK;
+    const size_t layer = (size_t)B * S * 3 * d;
+    const float *hi = (const float*)m.rows.p, *lo = hi + layer * m.cache.layers;
+    for (int l = 0; l < m.cache.layers && good; ++l, hi += layer, lo += layer)
+        good = gbx_kv_append(&m.cache, l, (const int32_t*)m.step.p, (int)most, ints + 2 * n, ints + 2 * n + B, B, S, hi + d, lo + d,
+                             hi + 2 * d, lo + 2 * d, 3 * d, m.err, gs) == GBX_OK;
+    good = good && cudaMemcpyAsync(&bits, m.err, 4, cudaMemcpyDeviceToHost, m.stream) == cudaSuccess &&
+           cudaStreamSynchronize(m.stream) == cudaSuccess && !bits;
+    return good || fail(std::string("session: the accepted tokens could not be kept: ") + gbx_last_error());
 }
 
 std::vector<float> Session::forward(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts,
@@ -518,7 +574,7 @@ bool Session::verify(const std::vector<int>& seqs, const std::vector<int>& ids, 
     Undo undo(*this);
     std::vector<int64_t> before;
     for (int s : seqs) before.push_back(table_.length(s));
-    if (!step(seqs, given, counts, true, padded, S)) return false;
+    if (!step(seqs, given, counts, true, padded, S, steps > 0)) return false;
     uint8_t* p = (uint8_t*)m.select.p;
     std::vector<int32_t> out(B * (size_t)S), acc(B);
     bool good = cudaMemcpyAsync(p, du.data(), du.size() * 8, cudaMemcpyHostToDevice, m.stream) == cudaSuccess &&
@@ -539,11 +595,14 @@ bool Session::verify(const std::vector<int>& seqs, const std::vector<int>& ids, 
            cudaStreamSynchronize(m.stream) == cudaSuccess;
     if (!good || bits)
         return fail(good ? std::string("session: a logits row gives no distribution") : std::string("session: verification failed: ") + gbx_last_error());
+    std::vector<int> keep(B);
+    for (size_t b = 0; b < B; ++b) keep[b] = 1 + acc[b];
+    if (!keepOnly(seqs, before, counts, keep, S)) return false;
     outIds->assign(B * n1, -1);
     accepted->assign(acc.begin(), acc.end());
     for (size_t b = 0; b < B; ++b) {
         for (int j = 0; j < S; ++j) (*outIds)[b * n1 + j] = out[b * S + j];
-        table_.truncate(seqs[b], before[b] + 1 + acc[b]);
+        table_.truncate(seqs[b], before[b] + keep[b]);
     }
     undo.done = true;
     return true;

@@ -457,20 +457,22 @@ bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, f
         const Impl::Layer& L = m.layers[l];
         const Impl::LayerW& W = m.wpairs[l];
         if (l > 0) check(gbx_layernorm_pair(m.h.p, m.ln.p, m.ln_lo.p, L.ln1_g, L.ln1_b, N, d, 1e-5f, gs));
-        linear(m.ln.p, m.ln_lo.p, W.qkv, L.qkv_b, nullptr, m.qkv.p, m.qkv_lo.p, N, 3 * d, d, GBX_ACT_NONE);
+        float* qkv = step && step->rows ? step->rows + (int64_t)l * N * 3 * d : m.qkv.p;
+        float* qkv_lo = step && step->rows ? step->rowsLo + (int64_t)l * N * 3 * d : m.qkv_lo.p;
+        linear(m.ln.p, m.ln_lo.p, W.qkv, L.qkv_b, nullptr, qkv, qkv_lo, N, 3 * d, d, GBX_ACT_NONE);
         if (step)
-            check(gbx_kv_append(step->cache, l, step->table, step->maxPages, step->kvLen, step->nNew, batch, S, m.qkv.p + d,
-                                m.qkv_lo.p + d, m.qkv.p + 2 * d, m.qkv_lo.p + 2 * d, 3 * d, m.err, gs));
+            check(gbx_kv_append(step->cache, l, step->table, step->maxPages, step->kvLen, step->nNew, batch, S, qkv + d,
+                                qkv_lo + d, qkv + 2 * d, qkv_lo + 2 * d, 3 * d, m.err, gs));
         if (step && !(step->fresh && m.fused)) {
             // the new rows over everything cached, their own keys and values included
-            check(gbx_attn_cached(step->cache, l, m.qkv.p, m.qkv_lo.p, 3 * d, step->table, step->maxPages, step->kvLen,
+            check(gbx_attn_cached(step->cache, l, qkv, qkv_lo, 3 * d, step->table, step->maxPages, step->kvLen,
                                   step->nNew, batch, S, H, scale, m.attn.p, m.attn_lo.p, d, step->workspace,
                                   step->workspaceFloats, m.err, gs));
         } else if (m.fused) {
             // attn = softmax(mask(Q K^T / sqrt(hd))) V for every head of every
             // sequence in one launch, as a tf32 pair
-            check(gbx_attn_fused(m.qkv.p, m.qkv_lo.p, m.qkv.p + d, m.qkv_lo.p + d, 3 * d, m.qkv.p + 2 * d,
-                                 m.qkv_lo.p + 2 * d, m.attn.p, m.attn_lo.p, d, batch, S, H, hd, scale, 1, m.err, gs));
+            check(gbx_attn_fused(qkv, qkv_lo, qkv + d, qkv_lo + d, 3 * d, qkv + 2 * d,
+                                 qkv_lo + 2 * d, m.attn.p, m.attn_lo.p, d, batch, S, H, hd, scale, 1, m.err, gs));
         }
         for (int b0 = 0; !m.fused && !step && b0 < batch; b0 += m.score_group) {
             const int g = batch - b0 < m.score_group ? batch - b0 : m.score_group;

@@ -207,6 +207,7 @@ private:
         bool even;                 // every sequence has S tokens
         bool fresh;                // and starts here
         bool allRows;              // logits of every row, else of each sequence's last
+        float *rows, *rowsLo;      // QKV rows of every layer, kept there; NULL: not kept
     };
     // logits stay on the device; hidden_host (optional) receives forwardHidden's blocks
     bool runForward(const std::vector<int>& tokenIDs, int batch, float* hidden_host = nullptr,
@@ -303,7 +304,8 @@ public:
     // [seq][nDraft][vocab], may be null; u: nDraft + 1 draws each).  outIds
     // receives nDraft + 1 entries a sequence: the accepted drafts, the next
     // token, -1s; accepted the counts.  Each sequence keeps its pending token and
-    // its accepted drafts; the next token is the next pending one.
+    // its accepted drafts, and its cache is what appending those alone leaves; the
+    // next token is the next pending one.
     bool verify(const std::vector<int>& seqs, const std::vector<int>& ids, int nDraft, const std::vector<int>& draftLen,
                 const float* draftLogits, double temperature, const std::vector<double>& u, std::vector<int>* outIds,
                 std::vector<int>* accepted);
@@ -314,7 +316,9 @@ private:
     struct Undo;
     bool fail(const std::string& msg);
     bool step(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, bool allRows,
-              const std::vector<int>& padded, int S);
+              const std::vector<int>& padded, int S, bool keepRows = false);
+    bool keepOnly(const std::vector<int>& seqs, const std::vector<int64_t>& before, const std::vector<int>& counts,
+                  const std::vector<int>& keep, int S);
     bool check(const std::vector<int>& seqs, const std::vector<int>& ids, const std::vector<int>& counts, int* S,
                std::vector<int>* padded);
     TransformerModel& model_;

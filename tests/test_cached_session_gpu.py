@@ -110,3 +110,61 @@ def test_a_verification_that_is_refused_after_its_forward(gm, model):
             s.verify(seqs, rng.integers(0, 700, (3, 3)), temperature=1e300, u=np.full((3, 3), 0.5))
         assert [s.length(x) for x in seqs] == [3, 20, 3] and s.free_pages() == t.free_pages()
         follow(s, t, seqs, rng)
+
+
+def drafts_of(t, seqs, pending, k, right, rng):
+    """[n, k] drafts: the first right[i] as the target says them itself (found on a fork), the others random."""
+    out = rng.integers(0, 700, (len(seqs), k))
+    for i, x in enumerate(seqs):
+        f, tok = t.fork(x), int(pending[i])
+        for j in range(right[i]):
+            tok = int(t.forward([f], [[tok]])[0].argmax())
+            out[i, j] = tok
+        t.release(f)
+    return out
+
+
+@pytest.mark.parametrize("P", [16, 32, 64])
+@pytest.mark.parametrize("with_len", [False, True])
+def test_rejected_drafts_leave_nothing(gm, tmp_path, P, with_len):
+    """Of one layer, whose keys and values depend on nothing but their token and place: after a verification the cache is
+    what appending the pending token and the accepted drafts alone would have left, bit for bit.  Rejected drafts
+    stand in the kept tokens' page, in one they share with a fork, and over the border to pages of their own."""
+    model = model_with(gm, tmp_path / "one.gguf", lambda t: None, layers=1)
+    rng = np.random.default_rng(P + with_len)
+    s, t, seqs = pair(gm, model, [rng.integers(0, 700, n) for n in (3, 13, 30, 16)], P, 60)
+    seqs.append(s.fork(1))
+    assert t.fork(1) == seqs[4]
+    k, counts = 4, set()
+    for step in range(8):
+        pending = rng.integers(0, 700, len(seqs))
+        drafts = drafts_of(t, seqs, pending, k, rng.integers(0, k + 1, len(seqs)), rng)
+        lens = rng.integers(0, k + 1, len(seqs)) if with_len else np.full(len(seqs), k)
+        out, acc = s.verify(seqs, np.concatenate([pending[:, None], drafts], 1), draft_len=lens)
+        counts.update((lens - acc).tolist())
+        kept = [np.concatenate([pending[i:i + 1], drafts[i, :acc[i]]]) for i in range(len(seqs))]
+        t.forward(seqs, kept)
+        assert [s.length(x) for x in seqs] == [t.length(x) for x in seqs] and s.free_pages() == t.free_pages()
+        follow(s, t, seqs, rng, 1)
+    assert 0 in counts and len(counts) > 1      # with and without rejected drafts
+
+
+def test_a_large_rejected_draft_does_not_coarsen_the_kept_tokens(gm, tmp_path):
+    """A token whose keys and values are many times the others', drafted and rejected time and again: the page's scales
+    stay those of the kept tokens, whose logits are a twin's that never saw it."""
+    def change(t):
+        t["blk.0.attn_norm.bias"][:] = 0
+        t["token_embd.weight"][699] = 0
+        t["token_embd.weight"][699, 5] = 50.0       # after the LayerNorm nearly all of the row is in one column
+        t["blk.0.attn_qkv.weight"][128:, 5] *= 10
+        t["output_norm.bias"][5] = -100             # its own logit (the tables are tied) far below the others
+    model = model_with(gm, tmp_path / "big.gguf", change, layers=1)
+    rng = np.random.default_rng(3)
+    s, t, seqs = pair(gm, model, [rng.integers(0, 699, 10)], 64)
+    for _ in range(6):
+        pending = int(rng.integers(0, 699))
+        out, acc = s.verify(seqs, [[pending, 699, 699]], temperature=0.5, u=np.full((1, 3), 1 - 2.0 ** -53))
+        assert acc[0] == 0
+        t.forward(seqs, [[pending]])
+        toks = rng.integers(0, 699, (1, 1))
+        same(s.forward(seqs, toks), t.forward(seqs, toks))
