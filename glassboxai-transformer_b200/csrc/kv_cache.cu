@@ -52,12 +52,25 @@ __device__ __forceinline__ float kv_new_scale(float a, bool bad)
 // max of the two, NaN where either is
 __device__ __forceinline__ float kv_max_scale(float a, float b) { return a != a || b != b ? a + b : fmaxf(a, b); }
 
-// An earlier code under a larger scale: the integer nearest to c * old / now.
-// The product has 31 bits and is exact in fp64, and the quotient of such
-// numbers is never so near a half that its fp64 rounding could cross it.
-__device__ __forceinline__ int kv_recode(int c, float old, float now)
+// Sixteen earlier codes under a larger scale, the first n of them: the integers
+// nearest to c * old / now, ties to even.  ratio is old / now rounded to fp64, so
+// c * ratio is off by less than 2^-44.  A quotient that is no tie keeps 2^-34 from one:
+// near a tie |c| old / now is about a half or more, so now's exponent is at most 9
+// above old's, and 2 c old - (odd) now is at least one unit of their 24 bits.  A tie
+// itself shows in the remainder, which is exact: c * old and q * now have 31 bits.
+__device__ __forceinline__ uint4 kv_recode16(uint4 w, int n, double old, double now, double ratio)
 {
-    return (int)rint((double)c * (double)old / (double)now);
+    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const double c = (double)(int8_t)(x[e >> 2] >> (8 * (e & 3)));
+        double q = rint(c * ratio);
+        const double rem = fma(-q, now, c * old), h = 0.5 * now;
+        if (fabs(rem) > h || (fabs(rem) == h && ((int)q & 1))) q += copysign(1.0, rem);
+        const uint32_t code = now > 0.0 ? (uint32_t)(int)q & 255u : 0u;
+        if (e < n) x[e >> 2] = (x[e >> 2] & ~(255u << (8 * (e & 3)))) | code << (8 * (e & 3));
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 struct KvRows {
@@ -129,9 +142,11 @@ __device__ __forceinline__ float4 kv_load4(const float* hi, const float* lo, int
     return x;
 }
 
-// The page's scale (old, where it holds earlier slots) with new values of
-// largest size amax in, and where it grew the codes of the slots before slot s0 recoded by `threads` threads, this one
-// the id-th.  Called by all of them, which have to meet before *scale is stored.
+// The page's scale (old, where it holds earlier slots) with new values of largest
+// size amax in, and where it grew the codes before slot s0 recoded by `threads`
+// threads, this one the id-th.  Called by all of them, which have to meet before
+// *scale is stored.  By words of 16 codes: one by one, a warp waited for memory some 80
+// times in a page of 40 tokens (32 sequences x 12 heads of width 64: 43 us a growing step, now 12).
 __device__ __forceinline__ float kv_grow(const KvBlock& k, int8_t* codes, float old, float amax, bool bad, int which, int hd,
                                          int id, int threads)
 {
@@ -139,10 +154,12 @@ __device__ __forceinline__ float kv_grow(const KvBlock& k, int8_t* codes, float 
     if (k.s0 > 0) {
         s = kv_max_scale(old, s);
         if (s != old) {   // grew, or turned NaN
-            for (int e = id; e < k.s0 * hd; e += threads) {
-                const int t = e / hd, i = e % hd;
-                int8_t* p = codes + (which ? ((t >> 4) * hd + i) * 16 + (t & 15) : t * hd + i);
-                *p = (int8_t)(s > 0.0f ? kv_recode(*p, old, s) : 0);
+            // words of 16 codes: of one token, or of one column and 16 tokens, the last of which may be new slots'
+            const double ratio = (double)old / (double)s;
+            const int words = which ? ((k.s0 + 15) >> 4) * hd : k.s0 * hd >> 4;
+            for (int e = id; e < words; e += threads) {
+                uint4* p = reinterpret_cast<uint4*>(codes) + e;
+                *p = kv_recode16(*p, which ? k.s0 - 16 * (e / hd) : 16, (double)old, (double)s, ratio);
             }
         }
     }
