@@ -342,10 +342,9 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
     const size_t rowFloats = keepRows ? padded.size() * 3 * (size_t)model_.getEmbedDim() * m.cache.layers : 0;
     if (!m.rows.ensure(rowFloats * 8)) return fail("session: cudaMalloc of the step's rows failed");
     std::vector<int64_t> before;
-    bool even = true, empty = true;
+    bool even = true;
     for (size_t i = 0; i < seqs.size(); ++i) {
         before.push_back(table_.length(seqs[i]));
-        empty = empty && before[i] == 0;
         even = even && counts[i] == S;
     }
     PageTable::Copies copies;
@@ -359,20 +358,21 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
     std::vector<int32_t> partial;
     for (int b = 0; b < B; ++b)
         if (before[b] % table_.pageSize()) partial.push_back(table_.pagesOf(seqs[b])[(size_t)(before[b] / table_.pageSize())]);
-    // one array: table, lengths, counts, positions, the pairs of page copies, the partial pages and 0, 1, ..
+    // one array: table, lengths, counts, counts of the sequences that go on, positions, the pairs of page copies, the partial pages and 0, 1, ..
     const size_t nCopies = copies.src.size(), nPartial = partial.size();
-    std::vector<int32_t> host((size_t)B * most + 2 * (size_t)B + (size_t)B * S, 0);
+    std::vector<int32_t> host((size_t)B * most + 3 * (size_t)B + (size_t)B * S, 0);
     const size_t atCopies = host.size(), atPartial = atCopies + 2 * nCopies;
     host.insert(host.end(), copies.src.begin(), copies.src.end());
     host.insert(host.end(), copies.dst.begin(), copies.dst.end());
     host.insert(host.end(), partial.begin(), partial.end());
     for (size_t i = 0; i < nPartial; ++i) host.push_back((int32_t)i);
-    int32_t *kvLen = host.data() + (size_t)B * most, *nNew = kvLen + B, *pos = nNew + B;
+    int32_t *kvLen = host.data() + (size_t)B * most, *nNew = kvLen + B, *nGoing = nNew + B, *pos = nGoing + B;
     for (int b = 0; b < B; ++b) {
         const std::vector<int32_t>& pages = table_.pagesOf(seqs[b]);
         std::copy(pages.begin(), pages.end(), host.begin() + (size_t)b * most);
         kvLen[b] = (int32_t)table_.length(seqs[b]);
         nNew[b] = counts[b];
+        nGoing[b] = before[b] ? counts[b] : 0;
         for (int j = 0; j < counts[b]; ++j) pos[(size_t)b * S + j] = (int32_t)(before[b] + j);
     }
     const int64_t wsFloats = gbx_attn_cached_workspace(&m.cache, B, S, m.cache.heads, (int)most);
@@ -398,12 +398,18 @@ bool Session::step(const std::vector<int>& seqs, const std::vector<int>& ids, co
     st.maxPages = (int)most;
     st.kvLen = st.table + (size_t)B * most;
     st.nNew = st.kvLen + B;
-    st.posIds = st.nNew + B;
+    st.nGoing = st.nNew + B;
+    st.posIds = st.nGoing + B;
     st.workspace = (float*)m.ws.p;
     st.workspaceFloats = wsFloats;
     st.counts = counts;
     st.even = even;
-    st.fresh = even && empty;
+    st.allFresh = true;
+    for (int b = 0; b < B; ++b) {
+        if (before[b]) st.allFresh = false;
+        else if (!st.fresh.empty() && st.fresh.back().second == b) ++st.fresh.back().second;
+        else st.fresh.emplace_back(b, b + 1);
+    }
     st.allRows = allRows;
     st.rows = keepRows ? (float*)m.rows.p : nullptr;
     st.rowsLo = st.rows + rowFloats;

@@ -463,17 +463,23 @@ bool TransformerModel::runForward(const std::vector<int>& tokenIDs, int batch, f
         if (step)
             check(gbx_kv_append(step->cache, l, step->table, step->maxPages, step->kvLen, step->nNew, batch, S, qkv + d,
                                 qkv_lo + d, qkv + 2 * d, qkv_lo + 2 * d, 3 * d, m.err, gs));
-        if (step && !(step->fresh && m.fused)) {
+        if (step && !(step->allFresh && m.fused)) {
             // the new rows over everything cached, their own keys and values included
             check(gbx_attn_cached(step->cache, l, qkv, qkv_lo, 3 * d, step->table, step->maxPages, step->kvLen,
-                                  step->nNew, batch, S, H, scale, m.attn.p, m.attn_lo.p, d, step->workspace,
+                                  m.fused ? step->nGoing : step->nNew, batch, S, H, scale, m.attn.p, m.attn_lo.p, d, step->workspace,
                                   step->workspaceFloats, m.err, gs));
-        } else if (m.fused) {
-            // attn = softmax(mask(Q K^T / sqrt(hd))) V for every head of every
-            // sequence in one launch, as a tf32 pair
-            check(gbx_attn_fused(qkv, qkv_lo, qkv + d, qkv_lo + d, 3 * d, qkv + 2 * d,
-                                 qkv_lo + 2 * d, m.attn.p, m.attn_lo.p, d, batch, S, H, hd, scale, 1, m.err, gs));
         }
+        // attn = softmax(mask(Q K^T / sqrt(hd))) V for every head of every
+        // sequence in one launch, as a tf32 pair.  (Causal, so that rows of zeros behind a
+        // shorter prompt's end change none of its own.)
+        auto fused = [&](int b0, int b1) {
+            const int64_t in = (int64_t)b0 * S * 3 * d, out = (int64_t)b0 * S * d;
+            check(gbx_attn_fused(qkv + in, qkv_lo + in, qkv + in + d, qkv_lo + in + d, 3 * d, qkv + in + 2 * d, qkv_lo + in + 2 * d,
+                                 m.attn.p + out, m.attn_lo.p + out, d, b1 - b0, S, H, hd, scale, 1, m.err, gs));
+        };
+        if (m.fused && !step) fused(0, batch);
+        if (m.fused && step)
+            for (const auto& run : step->fresh) fused(run.first, run.second);
         for (int b0 = 0; !m.fused && !step && b0 < batch; b0 += m.score_group) {
             const int g = batch - b0 < m.score_group ? batch - b0 : m.score_group;
             const float* qh = m.qkv.p + (int64_t)b0 * S * 3 * d;

@@ -60,6 +60,7 @@
 #include <memory>
 #include <random>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "gbx.h"
@@ -205,7 +206,12 @@ private:
         int64_t workspaceFloats;
         std::vector<int> counts;   // host copy of nNew
         bool even;                 // every sequence has S tokens
-        bool fresh;                // and starts here
+        // Sequences that start here attend over this step's own keys and values where the
+        // fused attention is on: runs [first, last) of them, and the counts of the others (0
+        // for these), which attend over the cache.
+        std::vector<std::pair<int, int>> fresh;
+        bool allFresh;
+        const int32_t* nGoing;
         bool allRows;              // logits of every row, else of each sequence's last
         float *rows, *rowsLo;      // QKV rows of every layer, kept there; NULL: not kept
     };

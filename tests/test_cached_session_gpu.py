@@ -168,3 +168,36 @@ def test_a_large_rejected_draft_does_not_coarsen_the_kept_tokens(gm, tmp_path):
         t.forward(seqs, [[pending]])
         toks = rng.integers(0, 699, (1, 1))
         same(s.forward(seqs, toks), t.forward(seqs, toks))
+
+
+def test_a_prompt_does_not_depend_on_its_batch_mates(gm, model):
+    """Prompts of different lengths, and beside sequences that go on: each has the logits of the forward of it alone
+    (tests/test_model_gpu.py's bound for the model's arithmetic, 1e-5 + 1e-3 of the logit; the batches take other
+    contraction shapes), not those of its keys and values in 8 bits."""
+    rng = np.random.default_rng(12)
+    s, t = gm.Session(model, 60, 16), gm.Session(model, 60, 16)
+    prompts = [rng.integers(0, 700, n) for n in (50, 7, 33, 1, 64)]
+    alone = [model.forward(p).ravel() for p in prompts]
+
+    def as_alone(got, i):
+        assert np.all(np.abs(got - alone[i]) <= 1e-5 + 1e-3 * np.abs(alone[i])), np.abs(got - alone[i]).max()
+
+    seqs = [s.new() for _ in prompts]
+    for i, row in enumerate(s.forward(seqs, prompts)):
+        as_alone(row, i)
+    # 1, 3 and 4 start while 0 and 2 go on with several tokens; the ones that go on take the steps they take alone
+    mixed, single = [t.new() for _ in prompts], gm.Session(model, 60, 16)
+    lone = [single.new() for _ in prompts]
+    for sess, ids in ((t, mixed), (single, lone)):
+        for i in (0, 2):
+            sess.forward([ids[i]], [prompts[i]])
+    more = {0: rng.integers(0, 700, 3), 2: rng.integers(0, 700, 9)}
+    got = t.forward(mixed, [more.get(i, prompts[i]) for i in range(5)])
+    for i in range(5):
+        if i in more:
+            want = single.forward([lone[i]], [more[i]])[0]
+            # the 8-bit cache may round one value another way under another contraction shape
+            assert np.abs(got[i] - want).max() <= 2e-3 * np.abs(want).max()
+        else:
+            as_alone(got[i], i)
+    assert [t.length(x) for x in mixed] == [53, 7, 42, 1, 64]
