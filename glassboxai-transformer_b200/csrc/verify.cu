@@ -30,6 +30,8 @@
 // second factor by its Taylor polynomial of degree 4 (|r ln 2 / 128| < 0.0028:
 // remainder below 1.3e-15), the 128 roots computed into shared memory by
 // exp2(): ten fp64 instructions where the fp64 pipe is what bounds C.
+#include <atomic>
+
 #include "gbx_common.cuh"
 #include "kv_cache.cuh"
 #include "row_stats.cuh"
@@ -37,6 +39,7 @@
 namespace gbx {
 
 constexpr int kVfMaxDraft = 256;
+constexpr size_t kVfStatic = 8192;   // shared memory left to the kernel's own arrays, at least
 constexpr int kVfQuads = 2;      // 16-byte loads of a lane in one unit of A
 
 // A warp's run of the vocabulary, and a lane's neighbouring entries of it (odd:
@@ -480,12 +483,22 @@ template <int C, int W>
 static int vf_launch(const VfArgs& a, int64_t B, const DeviceInfo& di, cudaStream_t s)
 {
     const size_t stats = vf_stats(a.n, C, W) + 8, kept = vf_kept(a.vocab, C, W);
-    const bool keep = !a.greedy && stats + kept + 8192 <= (size_t)di.max_smem_optin;
+    const size_t largest = (size_t)di.max_smem_optin - kVfStatic;
+    const bool keep = !a.greedy && stats + kept <= largest;
     const size_t smem = stats + (keep ? kept : 0);
+    const int mode = a.greedy ? VF_GREEDY : keep ? VF_KEEP : VF_AGAIN;
     auto k = a.greedy ? verify_kernel<C, W, VF_GREEDY> : keep ? verify_kernel<C, W, VF_KEEP> : verify_kernel<C, W, VF_AGAIN>;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        (C > 8 && cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
-        return check_launch("gbx_verify_tokens: launch attributes");
+    // The limit is the kernel's on this device, not the call's: set once, to the largest, so that
+    // no call lowers it between another thread's setting and its launch.
+    static std::atomic<uint64_t> ready[3];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("gbx_verify_tokens: device");
+    if (!(ready[mode].load(std::memory_order_acquire) >> dev & 1)) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)largest) != cudaSuccess ||
+            (C > 8 && cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
+            return check_launch("gbx_verify_tokens: launch attributes");
+        ready[mode].fetch_or((uint64_t)1 << dev, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * C));
     cfg.blockDim = dim3(32 * W);

@@ -2,6 +2,9 @@
 draws on the border of an acceptance, whose two sides differ by the last bits of
 fp32 row sums.  Either side is right there; half of one and half of the other
 is not."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -9,6 +12,8 @@ import kv_oracle
 from test_kv_cache_gpu import dev, i32
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PKG = os.path.join(ROOT, "glassboxai-transformer_b200")
 
 
 def softmax(x, T):
@@ -83,3 +88,15 @@ def test_the_same_call_gives_the_same_tokens(gbx, cuda, B):
         acc = torch.full((B,), -9, dtype=torch.int32, device="cuda")
         gbx.verify_tokens(args[0], args[1], out, acc, B=B, n_draft=n, vocab=V, temperature=1.0, uniforms=args[3], draft_logits=args[2])
         assert np.array_equal(acc.cpu().numpy(), wacc) and np.array_equal(out.cpu().numpy(), want)
+
+
+def test_calls_of_different_sizes_from_two_threads(gbx, cuda, tmp_path):
+    """A call with many drafts and one with few, each on a thread of its own (tests/cpp/verify_threads.cpp): neither takes
+    the shared memory that the other's launch needs."""
+    exe = str(tmp_path / "verify_threads")
+    home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-I", os.path.join(ROOT, "include"), "-I", os.path.join(home, "include"),
+                    os.path.join(ROOT, "tests", "cpp", "verify_threads.cpp"), "-o", exe, "-L", PKG, "-lgbx", "-L", os.path.join(home, "lib64"),
+                    "-lcudart", "-lpthread", f"-Wl,-rpath,{PKG}:{home}/lib64"], check=True)
+    p = subprocess.run([exe, "20000"], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and p.stdout.split() == ["ok"], p.stdout + p.stderr
