@@ -370,21 +370,43 @@ class KVCache:
         self._ref = ctypes.byref(self._c)
 
 
-def _index(name, t):
-    """Address of an index array: a contiguous int32 tensor, an address or None."""
-    if t is None or isinstance(t, int):
+def _misplaced(name, t, dev, n):
+    """Refuses a tensor on another device than the call's, or one that ends before the n-th entry from its start (that
+    of its storage counts: it may be a view): the kernel would read an address that is not there."""
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the call runs on cuda:{dev}")
+    if t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < n:
+        raise ValueError(f"{name} ends after {t.numel()} entries of {n}")
+
+
+def _index(name, t, dev=-1, n=0):
+    """Address of an index array of n entries: a contiguous int32 tensor (looked at where the call runs on GPU `dev` >=
+    0), an address or None."""
+    if t is None or t.__class__ is int:
         return t
     if t.dtype is not _Torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor")
+    if dev >= 0 and (t.numel() < n or t.get_device() != dev):
+        _misplaced(name, t, dev, n)
     return t.data_ptr()
 
 
-def _floats(name, t, dtype=None):
-    """Address of an array of floats: an fp32 (or `dtype`) tensor, an address or None.  It may be a strided view."""
-    if t is None or isinstance(t, int):
+def _floats(name, t, dev, n, dtype=None, strided=False):
+    """Address of an fp32 (or `dtype`) tensor, an address or None.  Of a strided one, a view of rows for instance, n
+    entries of its storage are to follow; any other is to have n itself."""
+    if t is None or t.__class__ is int:
         return t
     if t.dtype is not (dtype or _Torch.float32):
         raise ValueError(f"{name} must be a {dtype or _Torch.float32} tensor")
+    if dev >= 0:
+        if t.is_contiguous():
+            if t.numel() < n or t.get_device() != dev:
+                _misplaced(name, t, dev, n)
+        elif strided and (t.stride()[-1] == 1 or t.shape[-1] <= 1):
+            if t.get_device() != dev or t.untyped_storage().nbytes() < 4 * (t.storage_offset() + n):
+                _misplaced(name, t, dev, n)
+        else:
+            raise ValueError(f"{name} must be contiguous" + (" in its last dimension" if strided else ""))
     return t.data_ptr()
 
 
@@ -394,13 +416,18 @@ def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_
     kv_len[b] - n_new[b] + i of sequence b.  max_pages: the table's row length
     (its last dimension when it is a tensor)."""
     dev = cache._dev
-    if _elsewhere(dev):
+    if dev >= 0 and dev != _Torch.device():
         return _there(dev, kv_append, cache, layer, k, v, table, kv_len, B=B, S=S, ld=ld, max_pages=max_pages, n_new=n_new,
                       k_lo=k_lo, v_lo=v_lo, err_flag=err_flag, stream=stream)
-    rc = _lib.gbx_kv_append(cache._ref, layer, _index("table", table), table.shape[-1] if max_pages is None else max_pages,
-                            _index("kv_len", kv_len), _index("n_new", n_new), B, S, _floats("k", k), _floats("k_lo", k_lo),
-                            _floats("v", v), _floats("v_lo", v_lo), ld,
-                            _p(err_flag), _stream_on(dev, stream))
+    if max_pages is None:
+        max_pages = table.shape[-1]
+    at = dev if B > 0 and S > 0 else -1
+    n = (B * S - 1) * ld + cache.heads * cache.hd if at >= 0 and n_new is None else 0   # with counts, rows behind a sequence's own need not be there
+    rc = _lib.gbx_kv_append(
+        cache._ref, layer, _index("table", table, at, B * max_pages), max_pages, _index("kv_len", kv_len, at, B),
+        _index("n_new", n_new, at, B), B, S, _floats("k", k, at, n, None, True), _floats("k_lo", k_lo, at, n, None, True),
+        _floats("v", v, at, n, None, True), _floats("v_lo", v_lo, at, n, None, True), ld, _index("err_flag", err_flag, at, 1),
+        _stream_on(dev, stream))
     if rc:
         _check(rc)
 
@@ -408,13 +435,17 @@ def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_
 def kv_read(cache, layer, table, kv_len, k_out, v_out, *, B, S, ld, max_pages=None, n=None, err_flag=None, stream=None):
     """The fp32 values of each sequence's last n[b] tokens (the mirror of kv_append)."""
     dev = cache._dev
-    if _elsewhere(dev):
+    if dev >= 0 and dev != _Torch.device():
         return _there(dev, kv_read, cache, layer, table, kv_len, k_out, v_out, B=B, S=S, ld=ld, max_pages=max_pages, n=n,
                       err_flag=err_flag, stream=stream)
-    rc = _lib.gbx_kv_read(cache._ref, layer, _index("table", table), table.shape[-1] if max_pages is None else max_pages,
-                          _index("kv_len", kv_len), _index("n", n), B, S, _floats("k_out", k_out),
-                          _floats("v_out", v_out), ld, _p(err_flag),
-                          _stream_on(dev, stream))
+    if max_pages is None:
+        max_pages = table.shape[-1]
+    at = dev if B > 0 and S > 0 else -1
+    need = (B * S - 1) * ld + cache.heads * cache.hd if at >= 0 and n is None else 0
+    rc = _lib.gbx_kv_read(
+        cache._ref, layer, _index("table", table, at, B * max_pages), max_pages, _index("kv_len", kv_len, at, B), _index("n", n, at, B),
+        B, S, _floats("k_out", k_out, at, need, None, True), _floats("v_out", v_out, at, need, None, True), ld,
+        _index("err_flag", err_flag, at, 1), _stream_on(dev, stream))
     if rc:
         _check(rc)
 
@@ -422,9 +453,10 @@ def kv_read(cache, layer, table, kv_len, k_out, v_out, *, B, S, ld, max_pages=No
 def kv_copy_pages(cache, src, dst, *, n, err_flag=None, stream=None):
     """Page dst[i] becomes page src[i], i < n, in every layer."""
     dev = cache._dev
-    if _elsewhere(dev):
+    if dev >= 0 and dev != _Torch.device():
         return _there(dev, kv_copy_pages, cache, src, dst, n=n, err_flag=err_flag, stream=stream)
-    rc = _lib.gbx_kv_copy_pages(cache._ref, _index("src", src), _index("dst", dst), n, _p(err_flag), _stream_on(dev, stream))
+    rc = _lib.gbx_kv_copy_pages(cache._ref, _index("src", src, dev, n), _index("dst", dst, dev, n), n, _index("err_flag", err_flag, dev, 1),
+                                _stream_on(dev, stream))
     if rc:
         _check(rc)
 
@@ -443,17 +475,23 @@ def attn_cached(cache, layer, q, out, table, kv_len, *, B, S, H, ld, ld_out, sca
                 out_lo=None, workspace=None, workspace_floats=None, err_flag=None, stream=None):
     """Attention of S rows per sequence over the cached tokens (see gbx.h)."""
     dev = cache._dev
-    if _elsewhere(dev):
+    if dev >= 0 and dev != _Torch.device():
         return _there(dev, attn_cached, cache, layer, q, out, table, kv_len, B=B, S=S, H=H, ld=ld, ld_out=ld_out, scale=scale,
                       max_pages=max_pages, n_new=n_new, q_lo=q_lo, out_lo=out_lo, workspace=workspace,
                       workspace_floats=workspace_floats, err_flag=err_flag, stream=stream)
     if workspace_floats is None:
         workspace_floats = workspace.numel() if hasattr(workspace, "numel") else 0
-    rc = _lib.gbx_attn_cached(cache._ref, layer, _floats("q", q), _floats("q_lo", q_lo), ld, _index("table", table),
-                              table.shape[-1] if max_pages is None else max_pages, _index("kv_len", kv_len),
-                              _index("n_new", n_new), B, S, H, scale, _floats("out", out), _floats("out_lo", out_lo),
-                              ld_out, _floats("workspace", workspace),
-                              workspace_floats, _p(err_flag), _stream_on(dev, stream))
+    if max_pages is None:
+        max_pages = table.shape[-1]
+    at = dev if B > 0 and S > 0 else -1
+    rows, width = (B * S - 1, H * cache.hd) if at >= 0 and n_new is None else (0, 0)
+    n, n_out = rows * ld + width, rows * ld_out + width
+    rc = _lib.gbx_attn_cached(
+        cache._ref, layer, _floats("q", q, at, n, None, True), _floats("q_lo", q_lo, at, n, None, True), ld,
+        _index("table", table, at, B * max_pages), max_pages, _index("kv_len", kv_len, at, B), _index("n_new", n_new, at, B), B, S, H,
+        scale, _floats("out", out, at, n_out, None, True), _floats("out_lo", out_lo, at, n_out, None, True), ld_out,
+        _floats("workspace", workspace, at, workspace_floats), workspace_floats, _index("err_flag", err_flag, at, 1),
+        _stream_on(dev, stream))
     if rc:
         _check(rc)
 
@@ -462,12 +500,16 @@ def verify_tokens(logits, draft_ids, out_ids, n_accepted, *, B, n_draft, vocab, 
                   draft_logits=None, draft_len=None, err_flag=None, stream=None):
     """Accepts drafted tokens against the target's logits and picks the next token (see gbx.h)."""
     dev = _device_of(logits)
-    if _elsewhere(dev):
+    if dev >= 0 and dev != _Torch.device():
         return _there(dev, verify_tokens, logits, draft_ids, out_ids, n_accepted, B=B, n_draft=n_draft, vocab=vocab,
                       temperature=temperature, uniforms=uniforms, draft_logits=draft_logits, draft_len=draft_len,
                       err_flag=err_flag, stream=stream)
-    rc = _lib.gbx_verify_tokens(_floats("logits", logits), _floats("draft_logits", draft_logits), _index("draft_ids", draft_ids), _index("draft_len", draft_len), B,
-                                n_draft, vocab, temperature, _floats("uniforms", uniforms, _Torch.float64), _index("out_ids", out_ids),
-                                _index("n_accepted", n_accepted), _p(err_flag), _stream_on(dev, stream))
+    at = dev if B > 0 and n_draft >= 0 else -1
+    rows = B * (n_draft + 1)
+    rc = _lib.gbx_verify_tokens(
+        _floats("logits", logits, at, rows * vocab), _floats("draft_logits", draft_logits, at, B * n_draft * vocab),
+        _index("draft_ids", draft_ids, at, B * n_draft), _index("draft_len", draft_len, at, B), B, n_draft, vocab, temperature,
+        _floats("uniforms", uniforms, at, rows, _Torch.float64), _index("out_ids", out_ids, at, rows), _index("n_accepted", n_accepted, at, B),
+        _index("err_flag", err_flag, at, 1), _stream_on(dev, stream))
     if rc:
         _check(rc)
