@@ -86,7 +86,7 @@ struct AcArgs {
     int64_t ld_out;
     float* ws;        // partial results of nsplit > 1
     float qscale;     // log2(e) / scale
-    int H, G;         // query heads, query heads per key head
+    int G;            // query heads per key head
     int nrb;          // row blocks per (sequence, key head)
     int nsplit;       // clusters per unit
     FastDiv by_heads, by_nrb, by_g, by_nsplit, by_hd;
@@ -585,14 +585,13 @@ struct AcMeet {
         asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     }
 
-    // The same for many rows (300 rows of 12 heads over 4000 tokens: 35 us
+    // The same for many rows of several CTAs (300 rows of 12 heads over 4000 tokens: 35 us
     // against 40).  The factors that bring the partial results to one maximum are formed once
     // a row; then every thread takes four columns of a row at a time.
     __device__ __forceinline__ void finish(const AcArgs& a, const AcUnit& u, uint32_t unit, int split, uint32_t rank, uint32_t csize, int threads)
     {
         constexpr int Q = HD / 4;
         const int nr = u.rows;
-        const bool alone = csize == 1 && a.nsplit == 1;
         for (int r = threadIdx.x; r < nr; r += threads) {
             float mx = m[r];
 #pragma unroll
@@ -614,10 +613,8 @@ struct AcMeet {
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < NW; ++w) acc = fma4s(*reinterpret_cast<const float4*>(o + (w * R + r) * HD + col), m[w * R + r], acc);
-            if (alone) ac_store4(a, ac_row(a, u, r, a.ld_out) + col, acc, l[NW * R + r]);
-            else *reinterpret_cast<float4*>(o + (NW * R + r) * HD + col) = acc;
+            *reinterpret_cast<float4*>(o + (NW * R + r) * HD + col) = acc;
         }
-        if (alone) return;
         asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
         auto at = [&](uint32_t p, const float* x) { return tc::mapa(tc::smem_u32(x), p); };
         auto peer = [&](uint32_t p, const float* x) -> float {
@@ -1307,7 +1304,6 @@ extern "C" int gbx_attn_cached(const gbx_kv_cache* cache_host, int layer, const 
     a.ld_out = ld_out;
     a.ws = workspace;
     a.qscale = (float)(1.4426950408889634 / (double)scale);
-    a.H = H;
     a.G = H / a.c.heads;
     a.nrb = p.nrb;
     a.nsplit = p.nsplit;

@@ -23,7 +23,6 @@ struct gbx_sharded {
 
 struct gbx_session {
     gbx::Session session;
-    int vocab;
 };
 
 // No exception leaves a C entry point: an allocation that fails is an error code.
@@ -230,7 +229,7 @@ gbx_session* gbx_session_open(gbx_model* m, int64_t pages, int page_size)
     }
     gbx_session* s = nullptr;
     const int rc = guarded("gbx_session_open", [&] {
-        s = new gbx_session{{m->model, pages, page_size}, m->model.getVocabSize()};
+        s = new gbx_session{{m->model, pages, page_size}};
         return GBX_OK;
     });
     if (rc == GBX_OK && !s->session.ok()) {

@@ -100,3 +100,21 @@ def test_calls_of_different_sizes_from_two_threads(gbx, cuda, tmp_path):
                     "-lcudart", "-lpthread", f"-Wl,-rpath,{PKG}:{home}/lib64"], check=True)
     p = subprocess.run([exe, "20000"], capture_output=True, text=True, timeout=300)
     assert p.returncode == 0 and p.stdout.split() == ["ok"], p.stdout + p.stderr
+
+
+@pytest.mark.parametrize("T", [0.3, 1.0, 1.7])
+def test_every_plain_sample_is_the_inversion_of_its_row(gbx, cuda, T):
+    """Rows without drafts: the token of every draw, but for draws within 1e-11 of a border of the running sum."""
+    import torch
+    rng = np.random.default_rng(int(10 * T))
+    B, V = 300, 5001
+    logits = (rng.standard_normal((B, 1, V)) * 3).astype(np.float32)
+    p, u = softmax(logits, T), rng.random((B, 1))
+    out = torch.full((B, 1), -9, dtype=torch.int32, device="cuda")
+    acc = torch.full((B,), -9, dtype=torch.int32, device="cuda")
+    gbx.verify_tokens(dev(logits), None, out, acc, B=B, n_draft=0, vocab=V, temperature=T, uniforms=dev(u))
+    got = out.cpu().numpy()[:, 0]
+    assert not acc.cpu().numpy().any()
+    for b in range(B):
+        want, margin = next_of(p[b, 0], 0.0, False, u[b, 0])
+        assert got[b] == want or margin < 1e-11, (b, got[b], want, margin)
