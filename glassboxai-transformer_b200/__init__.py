@@ -392,8 +392,8 @@ def _index(name, t, dev=-1, n=0):
 
 
 def _floats(name, t, dev, n, dtype=None, strided=False):
-    """Address of an fp32 (or `dtype`) tensor, an address or None.  Of a strided one, a view of rows for instance, n
-    entries of its storage are to follow; any other is to have n itself."""
+    """Address of an fp32 (or `dtype`) tensor with n entries of storage from its start, an address or None.  strided: it
+    may be a view of rows that lie further apart."""
     if t is None or t.__class__ is int:
         return t
     if t.dtype is not (dtype or _Torch.float32):

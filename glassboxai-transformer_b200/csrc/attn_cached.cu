@@ -37,10 +37,10 @@
 // pages; 16 hd bytes each) a step or two ahead of its arithmetic.  Legacy
 // mma.sync is the right form here: a tile has 1 to 8 useful rows and 64 keys
 // that are used once, where a tcgen05 tile wants 128 rows.  256 sequences x 25
-// heads x 2048 tokens take 254 us (6.6 TB/s, the measured copy rate) in a burst
-// and 311 under the power cap, where the lower clock brings the arithmetic (230
-// us from L2) near the copies (239 alone); 2 x 8 heads x 120,001 tokens of width
-// 128 with 4 query heads each take 88 us (5.6 TB/s).
+// heads x 2048 tokens take 255 us (6.6 TB/s, the measured copy rate) in a burst
+// and 309 under the power cap, where the lower clock brings the arithmetic (243
+// us from L2) near the copies; 2 x 8 heads x 120,001 tokens of width 128 with 4
+// query heads each take 88 to 94 us (5.6 to 5.2 TB/s).
 //
 // A cluster of CTAs shares one (sequence, key head, row block): its warps take
 // the 64-token steps in turn and meet in shared memory, the CTAs through

@@ -169,8 +169,8 @@ __device__ __forceinline__ float kv_grow(const KvBlock& k, int8_t* codes, float 
 // Few new rows per sequence (a decode step, drafts): one warp per (sequence, block, K or V, head), the
 // largest |x| of the block's new rows, the scale, the codes.  The first 512
 // values are held in registers, others read again from L1.  Latency bounds it
-// (length, rows and page, scale, codes one after another): 3.3 us for 32 sequences x
-// 12 heads, 8.8 for 256 x 25.
+// (length, rows and page, scale, codes one after another): 2.9 us for 32 sequences x
+// 12 heads, 8.6 for 256 x 25.
 template <bool VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppend a)
 {
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppend a)
 // maximum and the codes, so each row is read once.  Keys: a lane has four
 // columns of every other slot (16-byte loads, 4-byte stores, a row's in
 // line); values: two columns of all 16 slots, whose codes are two 16-byte words
-// of the 16-tokens-innermost layout.  HBM bounds it: 32.5 us for 8 prompts of 1024
+// of the 16-tokens-innermost layout.  HBM bounds it: 32.8 us for 8 prompts of 1024
 // rows of 25 heads x 64 (131 MB, 4.0 TB/s), the rest the CTAs' start.
 template <bool VEC>
 __global__ void __launch_bounds__(512) kv_append_pages_kernel(const KvAppend a)

@@ -553,8 +553,8 @@ extern "C" int gbx_verify_tokens(const float* logits, const float* draft_logits,
     a.out_ids = out_ids;
     a.n_accepted = n_accepted;
     a.err = err_flag;
-    // One sequence of 4 drafts, 16 and 64 of up to 7, vocabulary 50257: 16, 30 and 79 us with
-    // clusters of 16 CTAs of 8 warps, 19, 41 and 68 with 8 of 16, 26, 41 and 85 with 4 of 16.
+    // One sequence of 4 drafts, 16 and 64 of up to 7, vocabulary 50257: 16, 28 and 79 us with
+    // clusters of 16 CTAs of 8 warps, 19, 41 and 69 with 8 of 16, 26, 41 and 85 with 4 of 16.
     DeviceInfo di;
     if (device_info(&di) != GBX_OK) return GBX_ECUDA;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -507,9 +507,12 @@ enum { GBX_KV_BAD_PAGE = 8, GBX_KV_BAD_LEN = 16, GBX_KV_BAD_PAIR = 32, GBX_VERIF
  * plus s/2 for each later growth of its page's scale.  A NaN or an infinity
  * among the new values makes the page's scale NaN for that head, so that
  * every later read of that page and head gives NaN until it is started anew.
- * Exact arithmetic, so the result does not depend on the launch.  Pages that
- * two sequences of one call both append to are the caller's mistake (their
- * bytes are then unspecified).
+ * Exact arithmetic, so the result does not depend on the launch.  All of a
+ * call's rows in a page are rounded at one scale, so a row that attends after
+ * the call sees its own and earlier tokens at a scale that the rows after it
+ * may have raised (within half of that larger step).  Pages that two sequences
+ * of one call both append to are the caller's mistake (their bytes are then
+ * unspecified).
  */
 int gbx_kv_append(const gbx_kv_cache* cache_host, int layer, const int32_t* table, int max_pages,
                   const int32_t* kv_len, const int32_t* n_new, int B, int S, const float* k_hi, const float* k_lo,
@@ -550,8 +553,8 @@ int gbx_kv_copy_pages(const gbx_kv_cache* cache_host, const int32_t* src, const 
  * fixed point relative to its largest entry, a weight times its page's value
  * scale 23-bit relative to the largest such product that its row sees among 64
  * neighbouring tokens; sums inside those are exact, all others fp32.  The
- * result is that of fp32 attention over the cached values (up to 2^118 in
- * size) to within rounding.
+ * result is that of fp32 attention over the cached values (scales from 2^-107,
+ * the smallest gbx_kv_append stores, values up to 2^118) to within rounding.
  * A page read by a valid row whose scale is NaN gives NaN; a row that sees no
  * page that can be read gives 0.  out and out_lo must overlap neither each
  * other nor q.

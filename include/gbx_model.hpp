@@ -270,9 +270,9 @@ private:
 // the model's layers (gbx_kv_cache) and any number of sequences in it; a step
 // costs the new tokens only, where TransformerModel::forward runs the whole
 // prefix.  Keys and values are held in 8 bits (see gbx_kv_append), so logits
-// differ from forward's by that rounding; a prompt that starts its sequences
-// attends over its unrounded keys and values.  The model must outlive the
-// session (a model is loaded once: a second loadModel fails and changes nothing).
+// differ from forward's by that rounding; a prompt that starts its sequence
+// attends over its unrounded keys and values where the fused attention is on
+// (head width 64).  The model must outlive the session (a model is loaded once: a second loadModel fails and changes nothing).
 // A session is used by one thread at a time, as the model is.
 class Session {
 public:
