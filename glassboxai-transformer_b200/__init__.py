@@ -391,6 +391,15 @@ def _index(name, t, dev=-1, n=0):
     return t.data_ptr()
 
 
+def _flag(t, dev):
+    """Address of the status word: a tensor of at least its four bytes, an address or None."""
+    if t is None or t.__class__ is int:
+        return t
+    if dev >= 0 and (t.get_device() != dev or t.numel() * t.element_size() < 4):
+        _misplaced("err_flag", t, dev, -(-4 // t.element_size()))
+    return t.data_ptr()
+
+
 def _floats(name, t, dev, n, dtype=None, strided=False):
     """Address of an fp32 (or `dtype`) tensor with n entries of storage from its start, an address or None.  strided: it
     may be a view of rows that lie further apart."""
@@ -426,7 +435,7 @@ def kv_append(cache, layer, k, v, table, kv_len, *, B, S, ld, max_pages=None, n_
     rc = _lib.gbx_kv_append(
         cache._ref, layer, _index("table", table, at, B * max_pages), max_pages, _index("kv_len", kv_len, at, B),
         _index("n_new", n_new, at, B), B, S, _floats("k", k, at, n, None, True), _floats("k_lo", k_lo, at, n, None, True),
-        _floats("v", v, at, n, None, True), _floats("v_lo", v_lo, at, n, None, True), ld, _index("err_flag", err_flag, at, 1),
+        _floats("v", v, at, n, None, True), _floats("v_lo", v_lo, at, n, None, True), ld, _flag(err_flag, at),
         _stream_on(dev, stream))
     if rc:
         _check(rc)
@@ -445,7 +454,7 @@ def kv_read(cache, layer, table, kv_len, k_out, v_out, *, B, S, ld, max_pages=No
     rc = _lib.gbx_kv_read(
         cache._ref, layer, _index("table", table, at, B * max_pages), max_pages, _index("kv_len", kv_len, at, B), _index("n", n, at, B),
         B, S, _floats("k_out", k_out, at, need, None, True), _floats("v_out", v_out, at, need, None, True), ld,
-        _index("err_flag", err_flag, at, 1), _stream_on(dev, stream))
+        _flag(err_flag, at), _stream_on(dev, stream))
     if rc:
         _check(rc)
 
@@ -455,7 +464,7 @@ def kv_copy_pages(cache, src, dst, *, n, err_flag=None, stream=None):
     dev = cache._dev
     if dev >= 0 and dev != _Torch.device():
         return _there(dev, kv_copy_pages, cache, src, dst, n=n, err_flag=err_flag, stream=stream)
-    rc = _lib.gbx_kv_copy_pages(cache._ref, _index("src", src, dev, n), _index("dst", dst, dev, n), n, _index("err_flag", err_flag, dev, 1),
+    rc = _lib.gbx_kv_copy_pages(cache._ref, _index("src", src, dev, n), _index("dst", dst, dev, n), n, _flag(err_flag, dev),
                                 _stream_on(dev, stream))
     if rc:
         _check(rc)
@@ -490,7 +499,7 @@ def attn_cached(cache, layer, q, out, table, kv_len, *, B, S, H, ld, ld_out, sca
         cache._ref, layer, _floats("q", q, at, n, None, True), _floats("q_lo", q_lo, at, n, None, True), ld,
         _index("table", table, at, B * max_pages), max_pages, _index("kv_len", kv_len, at, B), _index("n_new", n_new, at, B), B, S, H,
         scale, _floats("out", out, at, n_out, None, True), _floats("out_lo", out_lo, at, n_out, None, True), ld_out,
-        _floats("workspace", workspace, at, workspace_floats), workspace_floats, _index("err_flag", err_flag, at, 1),
+        _floats("workspace", workspace, at, workspace_floats), workspace_floats, _flag(err_flag, at),
         _stream_on(dev, stream))
     if rc:
         _check(rc)
@@ -510,6 +519,6 @@ def verify_tokens(logits, draft_ids, out_ids, n_accepted, *, B, n_draft, vocab, 
         _floats("logits", logits, at, rows * vocab), _floats("draft_logits", draft_logits, at, B * n_draft * vocab),
         _index("draft_ids", draft_ids, at, B * n_draft), _index("draft_len", draft_len, at, B), B, n_draft, vocab, temperature,
         _floats("uniforms", uniforms, at, rows, _Torch.float64), _index("out_ids", out_ids, at, rows), _index("n_accepted", n_accepted, at, B),
-        _index("err_flag", err_flag, at, 1), _stream_on(dev, stream))
+        _flag(err_flag, at), _stream_on(dev, stream))
     if rc:
         _check(rc)

@@ -201,3 +201,68 @@ def test_a_prompt_does_not_depend_on_its_batch_mates(gm, model):
         else:
             as_alone(got[i], i)
     assert [t.length(x) for x in mixed] == [53, 7, 42, 1, 64]
+
+
+@pytest.mark.parametrize("P,seed", [(16, 1), (32, 2), (64, 3)])
+def test_random_steps_with_failures_between(gm, tmp_path, P, seed):
+    """Prompts, tokens, chunks, verifications, forks, truncations, releases and compactions of a one-layer model, with
+    failing steps in between, against a session that takes only what stood: the same bits at every step."""
+    model = model_with(gm, tmp_path / "one.gguf", lambda t: None, layers=1)
+    rng = np.random.default_rng(seed)
+    s, t, live = gm.Session(model, 90, P), gm.Session(model, 90, P), []
+
+    def fail():
+        seqs = [x for x in live if s.length(x) < 240 and rng.random() < 0.7] or live[:1]
+        kind = rng.integers(0, 3)
+        if kind == 0:
+            prev = gbx.set_first_wait_limit(0)
+            try:
+                with pytest.raises(gbx.GbxError, match="timed out"):
+                    s.forward(seqs, [rng.integers(0, 700, rng.integers(1, 6)) for _ in seqs])
+            finally:
+                gbx.set_first_wait_limit(prev)
+        elif kind == 1:
+            with pytest.raises(gbx.GbxError, match="temperature"):
+                s.verify(seqs, rng.integers(0, 700, (len(seqs), 4)), temperature=1e300, u=np.full((len(seqs), 4), 0.5))
+        else:
+            with pytest.raises(gbx.GbxError):
+                s.forward(seqs + [seqs[0]], [[1]] * (len(seqs) + 1))
+
+    for step in range(70):
+        if live and step % 3 == 1:
+            fail()
+        kind = rng.integers(0, 9)
+        ready = [x for x in live if s.length(x) < 235]
+        if not ready or (kind == 0 and len(live) < 6):
+            x = s.new()
+            assert t.new() == x
+            live.append(x)
+            p = rng.integers(0, 700, rng.integers(1, 40))
+            same(s.forward([x], [p]), t.forward([x], [p]))
+        elif kind == 1 and len(live) < 6:
+            x = int(rng.choice(live))
+            live.append(s.fork(x))
+            assert t.fork(x) == live[-1]
+        elif kind == 2 and len(live) > 2:
+            x = live.pop(int(rng.integers(0, len(live))))
+            s.release(x)
+            t.release(x)
+        elif kind == 3:
+            x = int(rng.choice(live))
+            n = int(rng.integers(0, s.length(x) + 1))
+            s.truncate(x, n)
+            t.truncate(x, n)
+        elif kind == 4:
+            s.compact()
+        elif kind in (5, 6):
+            pending = rng.integers(0, 700, len(ready))
+            drafts = drafts_of(t, ready, pending, 3, rng.integers(0, 4, len(ready)), rng)
+            out, acc = s.verify(ready, np.concatenate([pending[:, None], drafts], 1))
+            t.forward(ready, [np.concatenate([pending[i:i + 1], drafts[i, :acc[i]]]) for i in range(len(ready))])
+        else:
+            toks = [rng.integers(0, 700, 1 if kind == 7 else rng.integers(1, 5)) for _ in ready]
+            same(s.forward(ready, toks), t.forward(ready, toks))
+        assert [s.length(x) for x in live] == [t.length(x) for x in live] and s.free_pages() == t.free_pages()
+    for x in live:
+        if s.length(x) < 250:
+            follow(s, t, [x], rng, 1)
